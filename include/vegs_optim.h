@@ -38,6 +38,49 @@ typedef struct VrAdamTensor {
  * launch up to 64 tensors). */
 int vr_adam_step(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps, void* stream);
 
+/* ---- the global gradient norm over many tensors, and clipping.
+ * One gradient: n elements in memory, in any order (the norm and the scaling do not depend on it).  data: device pointer,
+ * aligned to its element; dtype: a VrDataType.  Entries with n == 0 are skipped. */
+enum VrDataType { VR_F32 = 0, VR_BF16 = 1, VR_F16 = 2 };
+typedef struct VrGradTensor {
+    void* data;
+    int64_t n;
+    int64_t dtype;
+} VrGradTensor;
+
+/* A gradient that exists only as SH factors (see vr_sh_grad_from_factors below, same fields): its dense row enters the norm
+ * without being written. */
+typedef struct VrShGradFactors {
+    const float* means3D;
+    const float* campos;
+    const float* factors;
+    int64_t factor_view_stride;
+    int32_t P, n_views, sh_degree;
+    float scale;
+} VrShGradFactors;
+
+/* norm[0] (fp32) = the norm of all of them together: norm_type 2: sqrt(sum g^2), norm_type 0: max |g|.  Squares and sums are
+ * taken in fp64, in an order that depends only on the sizes: the same gradients give the same bits on every rank and in
+ * every run.  A NaN anywhere gives NaN; no elements give 0.  `tensors` and `factors` are HOST arrays.
+ * scratch: vr_grad_norm_scratch_bytes(count, n_factors) bytes on the device, 8-byte aligned, free for reuse in stream order. */
+int64_t vr_grad_norm_scratch_bytes(int32_t count, int32_t n_factors);
+int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
+                 int32_t norm_type, float* norm, void* scratch, void* stream);
+
+/* In place, for every element: g *= min(1, max_norm / (norm[0] + 1e-6)), the product in fp32 and rounded once to the
+ * gradient's type.  A factor of exactly one writes nothing; a NaN norm makes every element NaN and an infinite one gives
+ * zeros (NaN where the element itself is infinite), as torch.nn.utils.clip_grad_norm_ does.  max_norm >= 0. */
+int vr_clip_grads(const VrGradTensor* tensors, int32_t count, const float* norm, float max_norm, void* stream);
+
+/* vr_grad_norm and vr_clip_grads in a row; a handful of small tensors takes one launch for both. */
+int vr_clip_grad_norm(const VrGradTensor* tensors, int32_t count, int32_t norm_type, float max_norm, float* norm,
+                      void* scratch, void* stream);
+
+/* vr_adam_step of the clipped gradients: every gradient is multiplied by the factor above where it is loaded, and is left
+ * as it was in memory.  norm: device, from vr_grad_norm. */
+int vr_adam_step_clipped(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps,
+                         const float* norm, float max_norm, void* stream);
+
 /* For every Gaussian with radii > 0:  xyz_gradient_accum += ||means2D_grad[:2]||;  denom += 1;
  * max_radii2D = max(max_radii2D, radii).  means2D_grad [P,3], radii int32 [P], the three statistics fp32 [P]. */
 int vr_densify_stats(const float* means2D_grad, const int32_t* radii, int32_t P, float* xyz_gradient_accum,
@@ -119,6 +162,12 @@ typedef struct VrShAdamTensor {
 int vr_sh_adam_step(const float* means3D, int32_t P, const float* campos, const float* factors, int32_t n_views,
                     int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale, const VrShAdamTensor* dc,
                     const VrShAdamTensor* rest, double beta1, double beta2, double eps, void* stream);
+
+/* The same with the gradient clipped as vr_adam_step_clipped's is (norm from vr_grad_norm with these factors among its). */
+int vr_sh_adam_step_clipped(const float* means3D, int32_t P, const float* campos, const float* factors, int32_t n_views,
+                            int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale, const VrShAdamTensor* dc,
+                            const VrShAdamTensor* rest, double beta1, double beta2, double eps, const float* norm,
+                            float max_norm, void* stream);
 
 #ifdef __cplusplus
 }

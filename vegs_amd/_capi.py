@@ -32,6 +32,7 @@ EXPORTS = ["vr_abi_version", "vr_last_error", "vr_forward", "vr_backward", "vr_b
            "vr_normal_guidance_forward", "vr_normal_guidance_backward", "vr_training_loss_forward", "vr_training_loss_backward", "vr_adam_step", "vr_densify_stats",
            "vr_densify_plan_words", "vr_densify_plan", "vr_densify_apply", "vr_reset_opacity",
            "vr_sh_grad_from_factors", "vr_sh_adam_step",
+           "vr_grad_norm_scratch_bytes", "vr_grad_norm", "vr_clip_grads", "vr_clip_grad_norm", "vr_adam_step_clipped", "vr_sh_adam_step_clipped",
            "vr_instances_forward", "vr_instances_backward", "vr_activations_forward", "vr_activations_backward",
            "vr_boxmodel_forward", "vr_boxmodel_backward", "vr_boxmodel_regularizer_grad",
            "vr_xgmi_create", "vr_xgmi_detach", "vr_xgmi_destroy", "vr_xgmi_layout", "vr_xgmi_window", "vr_xgmi_handle", "vr_xgmi_attach",
@@ -95,6 +96,15 @@ class VrDensifyTensor(C.Structure):
 class VrShAdamTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("lr", C.c_double),
                 ("step", C.c_int64)]
+
+
+# VrGradTensor {data, n, dtype} is three 64-bit words: lists of them cross as flat int64 arrays
+VR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # VrDataType
+
+
+class VrShGradFactors(C.Structure):
+    _fields_ = [("means3D", C.c_void_p), ("campos", C.c_void_p), ("factors", C.c_void_p), ("factor_view_stride", C.c_int64),
+                ("P", C.c_int32), ("n_views", C.c_int32), ("sh_degree", C.c_int32), ("scale", C.c_float)]
 
 
 class VrInstance(C.Structure):
@@ -216,6 +226,20 @@ def load():
     lib.vr_sh_adam_step.restype = C.c_int
     lib.vr_sh_adam_step.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
                                     C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp]
+    i64p = C.POINTER(C.c_int64)
+    lib.vr_grad_norm_scratch_bytes.restype = C.c_int64
+    lib.vr_grad_norm_scratch_bytes.argtypes = [i32, i32]
+    lib.vr_grad_norm.restype = C.c_int
+    lib.vr_grad_norm.argtypes = [i64p, i32, C.POINTER(VrShGradFactors), i32, i32, vp, vp, vp]
+    lib.vr_clip_grads.restype = C.c_int
+    lib.vr_clip_grads.argtypes = [i64p, i32, vp, C.c_float, vp]
+    lib.vr_clip_grad_norm.restype = C.c_int
+    lib.vr_clip_grad_norm.argtypes = [i64p, i32, i32, C.c_float, vp, vp, vp]
+    lib.vr_adam_step_clipped.restype = C.c_int
+    lib.vr_adam_step_clipped.argtypes = [C.POINTER(VrAdamTensor), i32, C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
+    lib.vr_sh_adam_step_clipped.restype = C.c_int
+    lib.vr_sh_adam_step_clipped.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
+                                            C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
     lib.vr_instances_forward.restype = C.c_int
     lib.vr_instances_forward.argtypes = [C.POINTER(VrInstance), i32, vp, vp, vp, vp]
     lib.vr_instances_backward.restype = C.c_int

@@ -1,0 +1,257 @@
+// gradnorm.hip -- the global gradient norm over many tensors, and clipping (include/vegs_optim.h).
+//
+//   norm = sqrt(sum over all tensors of g^2)   or   max |g|;      g *= min(1, max_norm / (norm + 1e-6))
+//
+// Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more, and only when the factor is
+// not one.  The squares are taken and added in fp64: a product of two fp32 values is exact there and neither overflows
+// nor vanishes, and the vector ALUs do 64-bit multiply-adds an order of magnitude faster than memory delivers operands.
+// No atomics: every workgroup writes one partial result and one last workgroup adds them in a fixed order, so that the ranks of a
+// job that hold the same gradients clip by the same bits.
+#include "../../include/vegs_optim.h"
+#include "vr_host.h"
+#include "vr_sh_factors.h"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace vr {
+
+constexpr int GN_MAX_T = 128;              // tensors per launch: the table is a kernel argument, 128 x 24 B of its 4 KB
+constexpr int GN_UNIT = 256 * 16 * 4;      // bytes a workgroup handles at a time: 256 threads x 16 B x 4
+constexpr int GN_GRID = 2048;              // workgroups of a launch at most: eight for each of the 256 CUs
+
+struct GradSeg {
+    void* data;
+    long n;
+    int unit0;             // first unit of this tensor
+    int dtype;
+};
+struct GradArgs {
+    GradSeg seg[GN_MAX_T];
+    int count, units;
+};
+
+__device__ __forceinline__ float grad_value(const void* p, long i, int dtype)
+{
+    if (dtype == VR_F32) return reinterpret_cast<const float*>(p)[i];
+    if (dtype == VR_BF16) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
+    return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ uint16_t to_bf16(float x)       // nearest, ties to even; NaN stays NaN
+{
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void grad_scale(void* p, long i, int dtype, float c)
+{
+    const float x = c * grad_value(p, i, dtype);
+    if (dtype == VR_F32) reinterpret_cast<float*>(p)[i] = x;
+    else if (dtype == VR_BF16) reinterpret_cast<uint16_t*>(p)[i] = to_bf16(x);
+    else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+
+// the norm's accumulator: a sum of squares, or the largest magnitude (a NaN, once met, stays)
+template <bool MAX>
+__device__ __forceinline__ double norm_add(double acc, float x)
+{
+    if (MAX) { const float m = (float)acc, y = fabsf(x); return (y > m || y != y) ? (double)y : acc; }
+    return fma((double)x, (double)x, acc);
+}
+template <bool MAX>
+__device__ __forceinline__ double norm_join(double a, double b)
+{
+    if (MAX) return (b > a || b != b) ? b : a;
+    return a + b;
+}
+// over the workgroup's waves, in a fixed order; the result is thread 0's.  lds: one double per wave
+template <bool MAX>
+__device__ __forceinline__ double norm_block(double acc, double* lds)
+{
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) acc = norm_join<MAX>(acc, __shfl_xor(acc, d, 64));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) acc = norm_join<MAX>(acc, lds[w]);
+    return acc;
+}
+template <bool MAX>
+__device__ __forceinline__ float norm_value(double acc) { return MAX ? (float)acc : (float)sqrt(acc); }
+
+__device__ __forceinline__ GradSeg grad_seg(const GradArgs& a, int unit)
+{
+    int t = 0, hi = a.count - 1;          // the last tensor whose first unit is <= unit (scalar binary search)
+    while (t < hi) {
+        const int mid = (t + hi + 1) >> 1;
+        if (unit >= a.seg[mid].unit0) t = mid; else hi = mid - 1;
+    }
+    return a.seg[t];
+}
+
+template <bool MAX>
+__global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restrict__ partial)
+{
+    __shared__ double lds[4];
+    double acc = 0.0;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const GradSeg s = grad_seg(a, unit);
+        const long per = GN_UNIT / (s.dtype == VR_F32 ? 4 : 2);
+        const long base = (long)(unit - s.unit0) * per, end = base + per < s.n ? base + per : s.n;
+        for (long i = base + threadIdx.x; i < end; i += 256) acc = norm_add<MAX>(acc, grad_value(s.data, i, s.dtype));
+    }
+    acc = norm_block<MAX>(acc, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+// One Gaussian per thread: its dense SH row is rebuilt in registers, from the same function the optimizer's kernel
+// steps with, and only its squares leave.
+template <bool MAX>
+__global__ void __launch_bounds__(256) k_sh_grad_norm(ShFactorArgs a, double* __restrict__ partial)
+{
+    __shared__ double lds[4];
+    double acc = 0.0;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < a.P; i += gridDim.x * 256) {
+        float g[SHF_ROW_MAX];
+#pragma unroll
+        for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = 0.0f;
+        sh_row_from_factors(a, i, g);
+#pragma unroll
+        for (int q = 0; q < SHF_ROW_MAX; ++q) acc = norm_add<MAX>(acc, a.scale * g[q]);
+    }
+    acc = norm_block<MAX>(acc, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+template <bool MAX>
+__global__ void __launch_bounds__(1024) k_grad_norm_finish(const double* __restrict__ partial, int n, float* __restrict__ norm)
+{
+    __shared__ double lds[16];
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) acc = norm_join<MAX>(acc, partial[i]);
+    acc = norm_block<MAX>(acc, lds);
+    if (threadIdx.x == 0) norm[0] = norm_value<MAX>(acc);
+}
+
+__global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, const float* __restrict__ norm, float max_norm)
+{
+    const float c = clip_factor(*norm, max_norm);
+    if (c == 1.0f) return;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        const GradSeg s = grad_seg(a, unit);
+        const long per = GN_UNIT / (s.dtype == VR_F32 ? 4 : 2);
+        const long base = (long)(unit - s.unit0) * per, end = base + per < s.n ? base + per : s.n;
+        for (long i = base + threadIdx.x; i < end; i += 256) grad_scale(s.data, i, s.dtype, c);
+    }
+}
+
+static int check_grads(const VrGradTensor* t, int32_t count)
+{
+    if (count < 0 || (count > 0 && !t)) { set_error("grad norm: bad tensor list"); return VR_ERR_INVALID_ARGUMENT; }
+    for (int i = 0; i < count; ++i) {
+        if (t[i].dtype < VR_F32 || t[i].dtype > VR_F16) { set_error("grad norm: tensor %d has an unknown type", i); return VR_ERR_INVALID_ARGUMENT; }
+        const uintptr_t element = t[i].dtype == VR_F32 ? 4 : 2;
+        // (one tensor's units are counted in 31 bits: 2^31 x 16 KB)
+        if (t[i].n < 0 || (t[i].n > 0 && (!t[i].data || ((uintptr_t)t[i].data & (element - 1)))) || t[i].n > (1ll << 40))
+            { set_error("grad norm: tensor %d with NULL or misaligned data or a bad size", i); return VR_ERR_INVALID_ARGUMENT; }
+    }
+    return VR_OK;
+}
+
+// the next launch's table: up to GN_MAX_T non-empty tensors from `first` on; returns the first one not consumed
+static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
+{
+    int next = first;
+    a.count = a.units = 0;
+    for (; next < count && a.count < GN_MAX_T; ++next) {
+        if (t[next].n == 0) continue;
+        const long units = (t[next].n * (t[next].dtype == VR_F32 ? 4 : 2) + GN_UNIT - 1) / GN_UNIT;
+        if (a.units + units > 0x3fffffff) break;
+        a.seg[a.count++] = GradSeg{t[next].data, (long)t[next].n, a.units, (int)t[next].dtype};
+        a.units += (int)units;
+    }
+    for (int i = a.count; i < GN_MAX_T; ++i) a.seg[i] = GradSeg{nullptr, 0, 0x7fffffff, 0};
+    return next;
+}
+
+template <bool MAX>
+static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
+                     float* norm, double* partial, hipStream_t s)
+{
+    int n = 0;
+    for (int first = 0; first < count;) {
+        GradArgs a;
+        first = fill_grads(tensors, first, count, a);
+        if (a.units == 0) continue;
+        const int grid = a.units < GN_GRID ? a.units : GN_GRID;
+        hipLaunchKernelGGL(k_grad_norm<MAX>, dim3(grid), dim3(256), 0, s, a, partial + n);
+        n += grid;
+    }
+    for (int i = 0; i < n_factors; ++i) {
+        const VrShGradFactors& f = factors[i];
+        ShFactorArgs a;
+        if (int rc = sh_factor_args(a, f.means3D, f.P, f.campos, f.factors, f.n_views, f.factor_view_stride, f.sh_degree,
+                                    (f.sh_degree + 1) * (f.sh_degree + 1), f.scale)) return rc;
+        if (f.P == 0) continue;
+        const int grid = cdiv(f.P, 256) < GN_GRID ? cdiv(f.P, 256) : GN_GRID;
+        hipLaunchKernelGGL(k_sh_grad_norm<MAX>, dim3(grid), dim3(256), 0, s, a, partial + n);
+        n += grid;
+    }
+    hipLaunchKernelGGL(k_grad_norm_finish<MAX>, dim3(1), dim3(1024), 0, s, (const double*)partial, n, norm);
+    if (hipGetLastError() != hipSuccess) { set_error("grad norm: kernel launch failed"); return VR_ERR_HIP; }
+    return VR_OK;
+}
+
+static int clip_grads(const VrGradTensor* tensors, int32_t count, const float* norm, float max_norm, hipStream_t s)
+{
+    for (int first = 0; first < count;) {
+        GradArgs a;
+        first = fill_grads(tensors, first, count, a);
+        if (a.units == 0) continue;
+        hipLaunchKernelGGL(k_clip_grads, dim3(a.units < GN_GRID ? a.units : GN_GRID), dim3(256), 0, s, a, norm, max_norm);
+    }
+    if (hipGetLastError() != hipSuccess) { set_error("clip: kernel launch failed"); return VR_ERR_HIP; }
+    return VR_OK;
+}
+
+}  // namespace vr
+
+using namespace vr;
+
+// (a launch takes fewer than GN_MAX_T tensors only when its units run out, at 16 TB of gradients)
+extern "C" int64_t vr_grad_norm_scratch_bytes(int32_t count, int32_t n_factors)
+{
+    const int64_t launches = (count > 0 ? (count + GN_MAX_T - 1) / GN_MAX_T : 0) + (n_factors > 0 ? n_factors : 0);
+    return (launches > 0 ? launches : 1) * GN_GRID * (int64_t)sizeof(double);
+}
+
+extern "C" int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
+                            int32_t norm_type, float* norm, void* scratch, void* stream)
+{
+    if (int rc = check_grads(tensors, count)) return rc;
+    if (n_factors < 0 || (n_factors > 0 && !factors) || !norm || !scratch || ((uintptr_t)scratch & 7) || (norm_type != 2 && norm_type != 0))
+        { set_error("grad norm: needs norm, 8-byte aligned scratch and norm_type 2 or 0 (largest magnitude)"); return VR_ERR_INVALID_ARGUMENT; }
+    for (int i = 0; i < n_factors; ++i) {                  // everything is checked before anything is launched
+        const VrShGradFactors& f = factors[i];
+        ShFactorArgs a;
+        if (int rc = sh_factor_args(a, f.means3D, f.P, f.campos, f.factors, f.n_views, f.factor_view_stride, f.sh_degree,
+                                    (f.sh_degree + 1) * (f.sh_degree + 1), f.scale)) return rc;
+    }
+    return norm_type == 2 ? grad_norm<false>(tensors, count, factors, n_factors, norm, (double*)scratch, (hipStream_t)stream)
+                          : grad_norm<true>(tensors, count, factors, n_factors, norm, (double*)scratch, (hipStream_t)stream);
+}
+
+extern "C" int vr_clip_grads(const VrGradTensor* tensors, int32_t count, const float* norm, float max_norm, void* stream)
+{
+    if (int rc = check_grads(tensors, count)) return rc;
+    if (!norm || !(max_norm >= 0.0f)) { set_error("clip: needs a norm and max_norm >= 0"); return VR_ERR_INVALID_ARGUMENT; }
+    return clip_grads(tensors, count, norm, max_norm, (hipStream_t)stream);
+}
+
+extern "C" int vr_clip_grad_norm(const VrGradTensor* tensors, int32_t count, int32_t norm_type, float max_norm, float* norm,
+                                 void* scratch, void* stream)
+{
+    if (!(max_norm >= 0.0f)) { set_error("clip: max_norm must not be negative or NaN"); return VR_ERR_INVALID_ARGUMENT; }
+    if (int rc = vr_grad_norm(tensors, count, nullptr, 0, norm_type, norm, scratch, stream)) return rc;
+    return clip_grads(tensors, count, norm, max_norm, (hipStream_t)stream);
+}

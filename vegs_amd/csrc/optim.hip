@@ -11,6 +11,7 @@
 
 #include "../../include/vegs_optim.h"
 #include "vr_host.h"
+#include "vr_sh_factors.h"
 
 namespace vr {
 
@@ -32,6 +33,8 @@ struct AdamArgs {
     AdamSeg seg[ADAM_MAX_T];
     int count;
     float one_minus_b1, b2, one_minus_b2;
+    const float* norm;       // CLIP: the global gradient norm and its bound (gradnorm.hip)
+    float max_norm;
 };
 
 __device__ __forceinline__ void adam_elem(float& p, float g, float& m, float& v, const AdamSeg& s, const AdamArgs& a)
@@ -42,15 +45,22 @@ __device__ __forceinline__ void adam_elem(float& p, float g, float& m, float& v,
     p = p - s.step_size * (m / denom);                     // param.addcdiv_(exp_avg, denom, value=-step_size)
 }
 
+// CLIP: every gradient is multiplied by clip_factor(*norm, max_norm) where it is loaded -- the clipped gradients of
+// vr_clip_grads without their 12 bytes per element (read, write, read again); a factor of one leaves the step bit for bit.
+// The blocks then run from the last tensor to the first: the norm's pass ended there, and what it read last (up to 256 MB of
+// the gradients) is still in the memory-side cache.
+template <bool CLIP>
 __global__ void __launch_bounds__(256) k_adam(AdamArgs a)
 {
-    int t = 0, hi = a.count - 1;          // the last tensor whose first block is <= blockIdx.x (scalar binary search)
+    const int block = CLIP ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+    const float c = CLIP ? clip_factor(*a.norm, a.max_norm) : 1.0f;
+    int t = 0, hi = a.count - 1;          // the last tensor whose first block is <= block (scalar binary search)
     while (t < hi) {
         const int mid = (t + hi + 1) >> 1;
-        if ((int)blockIdx.x >= a.seg[mid].block0) t = mid; else hi = mid - 1;
+        if (block >= a.seg[mid].block0) t = mid; else hi = mid - 1;
     }
     const AdamSeg s = a.seg[t];
-    const long base = (long)(blockIdx.x - s.block0) * ADAM_EPB;
+    const long base = (long)(block - s.block0) * ADAM_EPB;
     const bool vec = ((((uintptr_t)s.p | (uintptr_t)s.g | (uintptr_t)s.m | (uintptr_t)s.v) & 15) == 0);
     if (vec && base + ADAM_EPB <= s.n) {
         float4 p[4], g[4], m[4], v[4];
@@ -64,6 +74,7 @@ __global__ void __launch_bounds__(256) k_adam(AdamArgs a)
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            if (CLIP) g[j] = make_float4(c * g[j].x, c * g[j].y, c * g[j].z, c * g[j].w);
             adam_elem(p[j].x, g[j].x, m[j].x, v[j].x, s, a);
             adam_elem(p[j].y, g[j].y, m[j].y, v[j].y, s, a);
             adam_elem(p[j].z, g[j].z, m[j].z, v[j].z, s, a);
@@ -76,7 +87,7 @@ __global__ void __launch_bounds__(256) k_adam(AdamArgs a)
     } else {
         for (long o = base + threadIdx.x; o < base + ADAM_EPB && o < s.n; o += 256) {
             float p = s.p[o], m = s.m[o], v = s.v[o];
-            adam_elem(p, s.g[o], m, v, s, a);
+            adam_elem(p, CLIP ? c * s.g[o] : s.g[o], m, v, s, a);
             s.p[o] = p; s.m[o] = m; s.v[o] = v;
         }
     }
@@ -103,21 +114,6 @@ k_densify_stats(const float* __restrict__ g2d, const int32_t* __restrict__ radii
 // exp_avg_sq in place (vr_sh_adam_step), so the 192-byte gradient row never exists in HBM.  Rows of the whole
 // [P,M,3] tensor are parked at stride 3M + 1 (odd for even M: bank-conflict free); with split storage the rest rows use
 // stride 3(M-1) + 1 and the DC row is handled by its own lane.
-constexpr int SHF_ROW_MAX = 48;
-struct ShAdamSeg {
-    float* p; float* m; float* v;          // Adam mode
-    float* out;                            // store mode
-    float step_size, inv_bc2_sqrt;
-};
-struct ShFactorArgs {
-    const float* means3D; const float* campos; const float* factors;
-    long view_stride;                      // floats between the factor blocks of consecutive views (3 P when packed)
-    int P, n_views, deg, M;
-    float scale;
-    ShAdamSeg dc, rest;                    // rest.p / rest.out == nullptr: `dc` is the whole [P,M,3] tensor
-    float one_minus_b1, b2, one_minus_b2, eps;
-};
-
 template <bool ADAM>
 __device__ __forceinline__ void sh_consume(const ShFactorArgs& a, const ShAdamSeg& s, size_t e, float g)
 {
@@ -180,7 +176,7 @@ __device__ __forceinline__ void sh_walk(const ShFactorArgs& a, const ShAdamSeg& 
     }
 }
 
-template <bool ADAM>
+template <bool ADAM, bool CLIP>
 __global__ void __launch_bounds__(256) k_sh_factors(ShFactorArgs a)
 {
     __shared__ float rows[4][64 * (SHF_ROW_MAX + 1)];
@@ -190,41 +186,28 @@ __global__ void __launch_bounds__(256) k_sh_factors(ShFactorArgs a)
     const int i = wave_first + lane;
     const int rows_here = min(64, a.P - wave_first);
     const bool split = ADAM ? a.rest.p != nullptr : a.rest.out != nullptr;
-    const int K = (a.deg + 1) * (a.deg + 1);
     float g[SHF_ROW_MAX];
 #pragma unroll
     for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = 0.0f;
-    if (i < a.P) {
-        const float px = a.means3D[3 * (size_t)i], py = a.means3D[3 * (size_t)i + 1], pz = a.means3D[3 * (size_t)i + 2];
-        for (int v = 0; v < a.n_views; ++v) {
-            const float* f = a.factors + (size_t)v * a.view_stride + (size_t)i * 3;
-            const float f0 = f[0], f1 = f[1], f2v = f[2];
-            if (f0 == 0.0f && f1 == 0.0f && f2v == 0.0f) continue;      // not visible in this view (or fully clamped)
-            const float d0 = px - a.campos[3 * v], d1 = py - a.campos[3 * v + 1], d2 = pz - a.campos[3 * v + 2];
-            const float il = 1.0f / sqrtf(d0 * d0 + d1 * d1 + d2 * d2);
-            float bas[16];
-            sh_basis(a.deg, d0 * il, d1 * il, d2 * il, bas);
+    if (i < a.P) sh_row_from_factors(a, i, g);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                if (k < K) {
-                    g[3 * k + 0] = fmaf(bas[k], f0, g[3 * k + 0]);
-                    g[3 * k + 1] = fmaf(bas[k], f1, g[3 * k + 1]);
-                    g[3 * k + 2] = fmaf(bas[k], f2v, g[3 * k + 2]);
-                }
-            }
-        }
+    for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = a.scale * g[q];
+    if (CLIP) {
+        const float c = clip_factor(*a.norm, a.max_norm);
+#pragma unroll
+        for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = c * g[q];
     }
     const int row = 3 * a.M;
     if (split) {
         if (i < a.P) {
 #pragma unroll
-            for (int c = 0; c < 3; ++c) sh_consume<ADAM>(a, a.dc, 3 * (size_t)i + c, a.scale * g[c]);
+            for (int c = 0; c < 3; ++c) sh_consume<ADAM>(a, a.dc, 3 * (size_t)i + c, g[c]);
         }
         const int rowr = row - 3, stride = rowr + 1;
         float* my = rows[w] + lane * stride;
 #pragma unroll
         for (int q = 0; q < SHF_ROW_MAX - 3; ++q)
-            if (q < rowr) my[q] = a.scale * g[3 + q];
+            if (q < rowr) my[q] = g[3 + q];
         __builtin_amdgcn_wave_barrier();
         sh_walk<ADAM>(a, a.rest, (size_t)wave_first * rowr, rows_here * rowr, rowr, stride, rows[w], lane);
     } else {
@@ -232,13 +215,13 @@ __global__ void __launch_bounds__(256) k_sh_factors(ShFactorArgs a)
         float* my = rows[w] + lane * stride;
 #pragma unroll
         for (int q = 0; q < SHF_ROW_MAX; ++q)
-            if (q < row) my[q] = a.scale * g[q];
+            if (q < row) my[q] = g[q];
         __builtin_amdgcn_wave_barrier();
         sh_walk<ADAM>(a, a.dc, (size_t)wave_first * row, rows_here * row, row, stride, rows[w], lane);
     }
 }
 
-static int sh_factor_args(ShFactorArgs& a, const float* means3D, int32_t P, const float* campos, const float* factors,
+int sh_factor_args(ShFactorArgs& a, const float* means3D, int32_t P, const float* campos, const float* factors,
                           int32_t n_views, int64_t view_stride, int32_t sh_degree, int32_t M, float scale)
 {
     if (view_stride != 0 && view_stride < 3 * (int64_t)P)
@@ -252,6 +235,8 @@ static int sh_factor_args(ShFactorArgs& a, const float* means3D, int32_t P, cons
     a.dc = ShAdamSeg{nullptr, nullptr, nullptr, nullptr, 0.f, 0.f};
     a.rest = a.dc;
     a.one_minus_b1 = a.b2 = a.one_minus_b2 = a.eps = 0.f;
+    a.norm = nullptr;
+    a.max_norm = 0.f;
     return VR_OK;
 }
 
@@ -270,14 +255,15 @@ extern "C" int vr_sh_grad_from_factors(const float* means3D, int32_t P, const fl
     if (!dL_dshs || (dL_dshs_rest && M < 2)) { set_error("sh factors: dL_dshs is required (and M >= 2 for split storage)"); return VR_ERR_INVALID_ARGUMENT; }
     a.dc.out = dL_dshs;
     a.rest.out = dL_dshs_rest;
-    hipLaunchKernelGGL(k_sh_factors<false>, dim3(cdiv(P, 256)), dim3(256), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_sh_factors<false, false>), dim3(cdiv(P, 256)), dim3(256), 0, (hipStream_t)stream, a);
     if (hipGetLastError() != hipSuccess) { set_error("sh factors: kernel launch failed"); return VR_ERR_HIP; }
     return VR_OK;
 }
 
-extern "C" int vr_sh_adam_step(const float* means3D, int32_t P, const float* campos, const float* factors, int32_t n_views,
-                               int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale, const VrShAdamTensor* dc,
-                               const VrShAdamTensor* rest, double beta1, double beta2, double eps, void* stream)
+static int sh_adam_step(const float* means3D, int32_t P, const float* campos, const float* factors, int32_t n_views,
+                        int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale, const VrShAdamTensor* dc,
+                        const VrShAdamTensor* rest, double beta1, double beta2, double eps, const float* norm, float max_norm,
+                        void* stream)
 {
     ShFactorArgs a;
     int rc = sh_factor_args(a, means3D, P, campos, factors, n_views, factor_view_stride, sh_degree, M, scale);
@@ -298,13 +284,36 @@ extern "C" int vr_sh_adam_step(const float* means3D, int32_t P, const float* cam
     a.b2 = (float)beta2;
     a.one_minus_b2 = (float)(1.0 - beta2);
     a.eps = (float)eps;
-    hipLaunchKernelGGL(k_sh_factors<true>, dim3(cdiv(P, 256)), dim3(256), 0, (hipStream_t)stream, a);
+    a.norm = norm;
+    a.max_norm = max_norm;
+    if (norm)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_sh_factors<true, true>), dim3(cdiv(P, 256)), dim3(256), 0, (hipStream_t)stream, a);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_sh_factors<true, false>), dim3(cdiv(P, 256)), dim3(256), 0, (hipStream_t)stream, a);
     if (hipGetLastError() != hipSuccess) { set_error("sh adam: kernel launch failed"); return VR_ERR_HIP; }
     return VR_OK;
 }
 
+extern "C" int vr_sh_adam_step(const float* means3D, int32_t P, const float* campos, const float* factors, int32_t n_views,
+                               int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale, const VrShAdamTensor* dc,
+                               const VrShAdamTensor* rest, double beta1, double beta2, double eps, void* stream)
+{
+    return sh_adam_step(means3D, P, campos, factors, n_views, factor_view_stride, sh_degree, M, scale, dc, rest, beta1, beta2,
+                        eps, nullptr, 0.0f, stream);
+}
 
-extern "C" int vr_adam_step(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps, void* stream)
+extern "C" int vr_sh_adam_step_clipped(const float* means3D, int32_t P, const float* campos, const float* factors,
+                                       int32_t n_views, int64_t factor_view_stride, int32_t sh_degree, int32_t M, float scale,
+                                       const VrShAdamTensor* dc, const VrShAdamTensor* rest, double beta1, double beta2,
+                                       double eps, const float* norm, float max_norm, void* stream)
+{
+    if (!norm || !(max_norm >= 0.0f)) { set_error("sh adam: the clipped step needs a norm and max_norm >= 0"); return VR_ERR_INVALID_ARGUMENT; }
+    return sh_adam_step(means3D, P, campos, factors, n_views, factor_view_stride, sh_degree, M, scale, dc, rest, beta1, beta2,
+                        eps, norm, max_norm, stream);
+}
+
+static int adam_step(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps, const float* norm,
+                     float max_norm, void* stream)
 {
     if (count < 0 || (count > 0 && !tensors)) { set_error("adam: bad tensor list"); return VR_ERR_INVALID_ARGUMENT; }
     for (int i = 0; i < count; ++i) {
@@ -321,6 +330,8 @@ extern "C" int vr_adam_step(const VrAdamTensor* tensors, int32_t count, double b
         a.one_minus_b1 = (float)(1.0 - beta1);
         a.b2 = (float)beta2;
         a.one_minus_b2 = (float)(1.0 - beta2);
+        a.norm = norm;
+        a.max_norm = max_norm;
         int blocks = 0;
         for (next = first; next < count && a.count < ADAM_MAX_T; ++next) {
             const VrAdamTensor& t = tensors[next];
@@ -337,10 +348,25 @@ extern "C" int vr_adam_step(const VrAdamTensor* tensors, int32_t count, double b
         }
         for (int i = a.count; i < ADAM_MAX_T; ++i) a.seg[i] = AdamSeg{nullptr, nullptr, nullptr, nullptr, 0, 0.f, 0.f, 0x7fffffff, 0.f};
         if (blocks == 0) continue;
-        hipLaunchKernelGGL(k_adam, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+        if (norm)
+            hipLaunchKernelGGL(k_adam<true>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+        else
+            hipLaunchKernelGGL(k_adam<false>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
         if (hipGetLastError() != hipSuccess) { set_error("adam: kernel launch failed"); return VR_ERR_HIP; }
     }
     return VR_OK;
+}
+
+extern "C" int vr_adam_step(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps, void* stream)
+{
+    return adam_step(tensors, count, beta1, beta2, eps, nullptr, 0.0f, stream);
+}
+
+extern "C" int vr_adam_step_clipped(const VrAdamTensor* tensors, int32_t count, double beta1, double beta2, double eps,
+                                    const float* norm, float max_norm, void* stream)
+{
+    if (!norm || !(max_norm >= 0.0f)) { set_error("adam: the clipped step needs a norm and max_norm >= 0"); return VR_ERR_INVALID_ARGUMENT; }
+    return adam_step(tensors, count, beta1, beta2, eps, norm, max_norm, stream);
 }
 
 extern "C" int vr_densify_stats(const float* means2D_grad, const int32_t* radii, int32_t P, float* xyz_gradient_accum,

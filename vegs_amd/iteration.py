@@ -213,17 +213,22 @@ class Trainer:
 
     def __init__(self, sc, device, n_boxes=0, fused=True, box_points=8196, factored_sh=False, lrs=None,
                  optimise_boxes=False, world=1, rank=0, group=None, exchange="factored", schedule=None, seed=0,
-                 box_model_cls=None):
+                 box_model_cls=None, max_grad_norm=None):
         """factored_sh (fused variant): the op returns the 3-float factor of the SH gradient and Adam consumes it directly
         (optim.adam_step_sh_factored) -- the static model's dense [P,16,3] gradient is never written.  With box instances
         in frame the factor covers the concatenated op inputs: the static model's rows feed Adam, the instances' few
         thousand rows are rebuilt densely (optim.sh_grad_from_factors on their world-space means).
         optimise_boxes: the instances are InstanceModels with their own optimizers and BoxModels with learnable pose
         corrections, all stepped every iteration (train.py:254-275); False keeps them as plain leaf tensors (gradients only).
+        max_grad_norm: clip what every optimizer steps with to this global norm (static model, instance models, pose
+        corrections together; after the exchange, so every rank clips by the same factor).  The fused variant applies the
+        factor inside the Adam launches -- a factored SH gradient enters the norm from its factors --, the op-by-op one calls
+        torch.nn.utils.clip_grad_norm_.  The norm of the last iteration: self.last["grad_norm"].
         world / rank / group: the view-sharded job; exchange: "factored" (default: forces factored_sh), "dense", or
         "direct" (vegs_amd.xgmi: hand-written peer-to-peer exchange)."""
         from . import optim
         self.device, self.fused = device, fused
+        self.max_grad_norm = max_grad_norm
         self.world, self.rank, self.group, self.exchange = int(world), int(rank), group, exchange
         if exchange not in ("factored", "dense", "direct"):
             raise ValueError(f"exchange must be 'factored', 'dense' or 'direct' (got {exchange!r})")
@@ -496,18 +501,28 @@ class Trainer:
                 self.direct.check()
             # ---- densification / opacity reset on schedule, then the optimizers (train.py:283-320, :254-275)
             replaced = self._scheduled()
-            if self.factored_sh and "static" not in replaced:
+            opts = [self.opt] + [m.opt for m in self.instances] + [bm.optimizer for bm in self.box_models]
+            step_factors = self.factored_sh and "static" not in replaced
+            norm, clip = None, {}
+            if self.max_grad_norm is not None:
+                if self.fused:
+                    norm = optim.grad_norm(opts, sh_factors=[(self.p["xyz"].detach(), Cv, Fv[:, :P0], deg, 1.0 / n_total)]
+                                           if step_factors else ())
+                    clip = dict(max_grad_norm=self.max_grad_norm, grad_norm=norm) if norm.is_cuda else {}   # (no gradients: nothing to clip)
+                else:
+                    norm = torch.nn.utils.clip_grad_norm_([p for o in opts for g in o.param_groups for p in g["params"]],
+                                                          self.max_grad_norm)
+            if step_factors:
                 ev = self.sh_adam_events          # (benchmarks: a HIP event pair around the SH Adam launch, when armed)
                 if ev is not None:
                     ev.append((torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)))
                     ev[-1][0].record()
                 optim.adam_step_sh_factored(self.opt, self.p["f_dc"], self.p["f_rest"], self.p["xyz"].detach(), Cv,
-                                            Fv[:, :P0], deg, 1.0 / n_total)
+                                            Fv[:, :P0], deg, 1.0 / n_total, **clip)
                 if ev is not None:
                     ev[-1][1].record()
-            opts = [self.opt] + [m.opt for m in self.instances] + [bm.optimizer for bm in self.box_models]
             if self.fused:
-                optim.step_many(opts)               # ONE multi-tensor launch: static model, instance models, pose corrections
+                optim.step_many(opts, **clip)       # ONE multi-tensor launch: static model, instance models, pose corrections
             else:
                 for o in opts:
                     o.step()
@@ -520,7 +535,7 @@ class Trainer:
                 w.grad = None
                 for t in b.values():
                     t.grad = None
-        self.last = {"factors": Fv, "campos": Cv, "replaced": replaced}
+        self.last = {"factors": Fv, "campos": Cv, "replaced": replaced, "grad_norm": norm}
         return losses, pkgs, grads
 
     # ---- what must be identical on every rank after an iteration

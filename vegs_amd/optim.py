@@ -7,6 +7,9 @@ by fused HIP kernels (vegs_amd/csrc/optim.hip, C ABI include/vegs_optim.h):
   densify_and_prune(optimizer, ...)     scene/gaussian_model.py:384-403 with its clone / split / prune and the
                                         optimizer-state surgery (:278-351), as one planned gather
   reset_opacity(optimizer)              scene/gaussian_model.py:215-218
+  grad_norm(parameters) / clip_grad_norm_(parameters, max_norm)
+                                        the global norm of many gradients, and torch.nn.utils.clip_grad_norm_
+  step_many(optimizers, max_grad_norm)  the Adam step of the clipped gradients, without rewriting them
 
 `Adam` is a torch.optim.Optimizer: param_groups (with the reference's extra "name" keys) and the per-parameter
 state dict {"step", "exp_avg", "exp_avg_sq"} have torch's layout, because the reference's densification code
@@ -86,26 +89,188 @@ def _collect(optimizer, by_cfg, keep):
                                    float(group["lr"]), int(st["step"].item()), float(group["eps"])))
 
 
+def _grads_of(parameters):
+    """The gradients of `parameters` -- a tensor, an optimizer, or an iterable of either -- each one once.  (Two launches of
+    the scaling's workgroups on one gradient would race.)"""
+    if isinstance(parameters, (torch.Tensor, torch.optim.Optimizer)):
+        parameters = [parameters]
+    out = {}
+    for p in parameters:
+        for q in ([t for g in p.param_groups for t in g["params"]] if isinstance(p, torch.optim.Optimizer) else (p,)):
+            g = q.grad
+            if g is not None:
+                out[g.data_ptr(), g.numel()] = g
+    return list(out.values())
+
+
+def _dense(t):
+    """Whether the elements of `t` fill their memory without gaps or repeats, in whatever order (a norm or a scaling does
+    not care about the order)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _grad_table(grads):
+    """(flat VrGradTensor words, device) of validated gradients that fill their memory."""
+    flat, device, dtypes = [], grads[0].device, _capi.VR_DTYPES
+    for g in grads:
+        if g.device != device or not g.is_cuda:
+            raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
+        kind = dtypes.get(g.dtype)
+        if kind is None or g.layout != torch.strided:
+            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.dtype}, {g.layout})")
+        flat += (g.data_ptr(), g.numel(), kind)
+    return (C.c_int64 * len(flat))(*flat), device
+
+
+def _norm_kind(norm_type):
+    norm_type = float(norm_type)
+    if norm_type == 2.0:
+        return 2
+    if norm_type == math.inf:
+        return 0
+    raise NotImplementedError(f"norm_type {norm_type}: the 2-norm and the largest magnitude (inf) are supported")
+
+
+def _check_max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative or NaN (got {max_norm})")
+    return max_norm
+
+
+def _scratch(lib, count, n_factors, device):
+    return torch.empty(lib.vr_grad_norm_scratch_bytes(count, n_factors) >> 3, dtype=torch.float64, device=device)
+
+
+def grad_norm(parameters, norm_type=2.0, sh_factors=()):
+    """The norm of all gradients of `parameters` (a tensor, an optimizer, or an iterable of either) as if they were one
+    vector: a 0-dim float32 tensor on their device.  Squares and sums are taken in 64 bits in an order that depends on the
+    sizes only -- every rank that holds the same gradients gets the same bits.  Parameters without a gradient are skipped,
+    a gradient met twice counts once; no gradients at all give a zero on the CPU, as in torch.
+
+    norm_type: 2.0 or math.inf (the largest magnitude).  Gradients: float32, bfloat16 or float16.
+    sh_factors: gradients that exist only as factors, as (means3D, campos, factors, sh_degree, scale) -- the arguments of
+    adam_step_sh_factored, whose gradient enters the norm without being written."""
+    kind = _norm_kind(norm_type)
+    grads = _grads_of(parameters)
+    keep, items = [g if g.layout != torch.strided or _dense(g) else g.contiguous() for g in grads], []
+    for means3D, campos, factors, sh_degree, scale in sh_factors:
+        P, n, means3D, campos, factors, fstride = _check_factor_inputs(means3D, campos, factors)
+        if keep and means3D.device != keep[0].device or items and means3D.device != items[0][1].device:
+            raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
+        keep_f = (means3D, campos, factors)
+        items.append((_capi.VrShGradFactors(_capi.ptr(means3D), _capi.ptr(campos), _capi.ptr(factors), fstride, P, n,
+                                            int(sh_degree), float(scale)), means3D, keep_f))
+    if not keep and not items:
+        return torch.tensor(0.0)
+    table, device = _grad_table(keep) if keep else (None, items[0][1].device)
+    lib = _capi.load()
+    with torch.cuda.device(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        scratch = _scratch(lib, len(keep), len(items), device)
+        _capi.check(lib.vr_grad_norm(table, len(keep), (_capi.VrShGradFactors * len(items))(*[i[0] for i in items]), len(items),
+                                     kind, norm.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+    return norm
+
+
+_grad_norm = grad_norm                    # (an argument of step_many and adam_step_sh_factored has the function's name)
+
+
 @torch.no_grad()
-def step_many(optimizers):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
+    """torch.nn.utils.clip_grad_norm_ on the GPU: scales the gradients of `parameters` (a tensor, an optimizer, or an iterable
+    of either) in place by min(1, max_norm / (norm + 1e-6)) and returns their norm from before, a 0-dim float32 tensor.
+    The norm is grad_norm()'s.  Gradients below the bound are not written at all; a NaN norm makes all of them NaN, as in
+    torch; error_if_nonfinite=True waits for the norm and raises before anything is scaled.  `foreach` has no effect (there
+    is one path).  step_many(max_grad_norm=...) clips inside the Adam step instead and leaves the gradients alone."""
+    max_norm, kind = _check_max_norm(max_norm), _norm_kind(norm_type)
+    grads = _grads_of(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    copies = []
+    for i, g in enumerate(grads):
+        if g.layout == torch.strided and not _dense(g):
+            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+                raise ValueError("an expanded gradient (one value in memory for several elements) cannot be clipped in place")
+            grads[i] = g.contiguous()
+            copies.append((g, grads[i]))
+    table, device = _grad_table(grads)
+    lib = _capi.load()
+    with torch.cuda.device(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        scratch = _scratch(lib, len(grads), 0, device)
+        stream = torch.cuda.current_stream(device).cuda_stream
+        if error_if_nonfinite:
+            _capi.check(lib.vr_grad_norm(table, len(grads), None, 0, kind, norm.data_ptr(), scratch.data_ptr(), stream))
+            if not math.isfinite(norm.item()):
+                raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is not finite, so they cannot be "
+                                   "clipped; error_if_nonfinite=False scales them all the same")
+            _capi.check(lib.vr_clip_grads(table, len(grads), norm.data_ptr(), max_norm, stream))
+        else:
+            _capi.check(lib.vr_clip_grad_norm(table, len(grads), kind, max_norm, norm.data_ptr(), scratch.data_ptr(), stream))
+    for g, copy in copies:
+        g.copy_(copy)
+    return norm
+
+
+def _check_norm(norm, device):
+    if not isinstance(norm, torch.Tensor) or norm.device != device or norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError(f"grad_norm must be a float32 tensor of one value on {device} (what optim.grad_norm returns)")
+
+
+@torch.no_grad()
+def step_many(optimizers, max_grad_norm=None, grad_norm=None):
     """optimizer.step() of SEVERAL Adam optimizers as one launch (per 64 tensors): what train.py:254-275 does one optimizer
     after the other when dynamic objects are in frame -- the static model's six groups, six more per instance model
     (densification_and_optimization(..., box=True)) and the three pose corrections of every BoxModel
     (box_model.optimizer.step(), model/boxmodel.py:13) -- with every tensor's own learning rate, step count and eps in
     the kernel's block->tensor table.  Optimizers may be vegs_amd.optim.Adam or torch.optim.Adam (same state layout).
-    All-or-nothing: every optimizer is validated before any state (step counters, fresh moments) is touched."""
-    lib = _capi.load()
+    All-or-nothing: every optimizer is validated before any state (step counters, fresh moments) is touched.
+
+    max_grad_norm: step with the gradients clipped to this global norm, as if clip_grad_norm_ had been called on all the
+    optimizers together before -- but the factor is applied where Adam loads a gradient, and .grad keeps its values.
+    Returns the norm (0-dim float32 on the GPU) then.  grad_norm: that norm where the caller has it already, from
+    optim.grad_norm over these AND other gradients (one joint norm for several calls)."""
     optimizers = list(optimizers)
+    if max_grad_norm is None:
+        if grad_norm is not None:
+            raise ValueError("grad_norm without max_grad_norm")
+    else:
+        max_grad_norm = _check_max_norm(max_grad_norm)
+    lib = _capi.load()
     for opt in optimizers:
         _validate(opt)
+    norm = None
+    if max_grad_norm is not None:
+        devices = {p.device for opt in optimizers for g in opt.param_groups for p in g["params"] if p.grad is not None}
+        if len(devices) > 1:
+            raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
+        if grad_norm is not None:
+            for device in devices:
+                _check_norm(grad_norm, device)
+            norm = grad_norm
+        else:
+            norm = _grad_norm(optimizers)
     by_cfg, keep = {}, []
     for opt in optimizers:
         _collect(opt, by_cfg, keep)
     for (device, b1, b2), items in by_cfg.items():
         arr = (_capi.VrAdamTensor * len(items))(*items)
         with torch.cuda.device(device):
-            rc = lib.vr_adam_step(arr, len(items), b1, b2, -1.0, torch.cuda.current_stream(device).cuda_stream)
+            stream = torch.cuda.current_stream(device).cuda_stream
+            if norm is None:
+                rc = lib.vr_adam_step(arr, len(items), b1, b2, -1.0, stream)
+            else:
+                rc = lib.vr_adam_step_clipped(arr, len(items), b1, b2, -1.0, norm.data_ptr(), max_grad_norm, stream)
         _capi.check(rc)
+    return norm
 
 
 def add_densification_stats(viewspace_point_grad, radii, xyz_gradient_accum, denom, max_radii2D):
@@ -336,11 +501,20 @@ def _sh_state(opt, p):
 
 
 @torch.no_grad()
-def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, factors, sh_degree, scale=1.0):
+def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, factors, sh_degree, scale=1.0,
+                          max_grad_norm=None, grad_norm=None):
     """One Adam step of the SH parameters (features_dc [P,1,3] + features_rest [P,M-1,3], or the whole [P,M,3] tensor with
     features_rest=None) of optimizer `opt` (vegs_amd.optim.Adam or torch.optim.Adam: same state layout) straight from
     the factors -- the dense gradient is built per Gaussian in registers and never written.  Equivalent to setting
-    .grad = sh_grad_from_factors(...) on the two parameters and stepping only them."""
+    .grad = sh_grad_from_factors(...) on the two parameters and stepping only them.
+
+    max_grad_norm: clip this gradient as step_many does.  grad_norm: the joint norm (optim.grad_norm with this gradient among
+    its sh_factors); without it the norm is this gradient's own.  Returns the norm then."""
+    if max_grad_norm is None:
+        if grad_norm is not None:
+            raise ValueError("grad_norm without max_grad_norm")
+    else:
+        max_grad_norm = _check_max_norm(max_grad_norm)
     P, n, means3D, campos, factors, fstride = _check_factor_inputs(means3D, campos, factors)
     M = features_dc.shape[1] + (features_rest.shape[1] if features_rest is not None else 0)
     items, states, betas, eps = [], [], None, None
@@ -362,11 +536,20 @@ def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, fact
     if not 0 <= int(sh_degree) <= 3 or M < K:
         raise ValueError(f"sh_degree {sh_degree} needs {K} coefficients, the parameters hold {M}")
     dev = means3D.device
+    norm = None
+    if max_grad_norm is not None:
+        if grad_norm is not None:
+            _check_norm(grad_norm, dev)
+        norm = grad_norm if grad_norm is not None else _grad_norm((), sh_factors=[(means3D, campos, factors, sh_degree, scale)])
+    args = (_capi.ptr(means3D), P, _capi.ptr(campos), _capi.ptr(factors), n, fstride, int(sh_degree), int(M), float(scale),
+            C.byref(items[0]), C.byref(items[1]) if items[1] is not None else None, betas[0], betas[1], eps)
     with torch.cuda.device(dev):
-        rc = _capi.load().vr_sh_adam_step(_capi.ptr(means3D), P, _capi.ptr(campos), _capi.ptr(factors), n, fstride, int(sh_degree),
-                                          int(M), float(scale), C.byref(items[0]),
-                                          C.byref(items[1]) if items[1] is not None else None, betas[0], betas[1], eps,
-                                          torch.cuda.current_stream(dev).cuda_stream)
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if norm is None:
+            rc = _capi.load().vr_sh_adam_step(*args, stream)
+        else:
+            rc = _capi.load().vr_sh_adam_step_clipped(*args, norm.data_ptr(), max_grad_norm, stream)
     _capi.check(rc)
     for st in states:          # the step counters advance only once every check and the call itself have passed
         st["step"] += 1
+    return norm
