@@ -1,0 +1,75 @@
+"""CPU: the refusals of the row lookup, at the Python surface and at the C ABI."""
+import ctypes as C
+
+import pytest
+import torch
+
+from vegs_amd import _capi, embedding
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(ValueError, match="GPU"):
+        embedding.lookup(torch.zeros(4, 3), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="GPU"):
+        embedding.lookup([[1.0]], torch.zeros(2, dtype=torch.int64))
+
+
+def _lookup(**over):
+    some = 1 << 20                                        # (a made-up address: nothing is launched for a refused call)
+    args = dict(table=some, ids=some, row_scale=None, n=5, rows=7, width=3, table_stride=3, table_dtype=0, out_dtype=0, ids_64=0,
+                scale=1.0)
+    args.update(over)
+    return _capi.VrLookup(*[args[f] for f, _ in _capi.VrLookup._fields_])
+
+
+BAD = [dict(n=-1), dict(n=1 << 30), dict(rows=-1), dict(rows=0x7fffffff), dict(width=0), dict(width=(1 << 24) + 1),
+       dict(table_stride=2), dict(table_dtype=3), dict(table_dtype=-1), dict(out_dtype=1), dict(table_dtype=1, out_dtype=2),
+       dict(table=None), dict(ids=None), dict(table=(1 << 20) + 2), dict(ids=(1 << 20) + 4, ids_64=1), dict(ids=(1 << 20) + 2),
+       dict(row_scale=(1 << 20) + 1)]
+
+
+@pytest.mark.parametrize("over", BAD, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+def test_c_entries_refuse_bad_lookups(over):
+    lib = _capi.load()
+    some = 1 << 20
+    bad = _lookup(**over)
+    assert lib.vr_lookup_forward(C.byref(bad), some, None) == -1
+    assert b"lookup" in lib.vr_last_error()
+    assert lib.vr_lookup_backward(C.byref(bad), some, 3, some, None, some, 1 << 30, None) == -1
+
+
+def test_c_entries_refuse_bad_outputs_and_scratch():
+    lib = _capi.load()
+    some, good = 1 << 20, _lookup()
+    assert lib.vr_lookup_forward(None, some, None) == -1
+    assert lib.vr_lookup_forward(C.byref(good), None, None) == -1
+    assert lib.vr_lookup_forward(C.byref(good), some + 2, None) == -1
+    need = lib.vr_lookup_scratch_bytes(5, 7, 3)
+    assert need > 0
+    for grad, stride, d_table, d_scale, scratch, nbytes in ((None, 3, some, None, some, need), (some, 2, some, None, some, need),
+                                                            (some + 2, 3, some, None, some, need), (some, 3, some + 2, None, some, need),
+                                                            (some, 3, some, some + 2, some, need), (some, 3, some, None, None, need),
+                                                            (some, 3, some, None, some + 16, need), (some, 3, some, None, some, need - 1)):
+        assert lib.vr_lookup_backward(C.byref(good), grad, stride, d_table, d_scale, scratch, nbytes, None) == -1
+    for sizes in ((-1, 7, 3), (1 << 30, 7, 3), (5, -1, 3), (5, 0x7fffffff, 3), (5, 7, 0), (5, 7, (1 << 24) + 1)):
+        assert lib.vr_lookup_scratch_bytes(*sizes) == 0
+
+
+def test_nothing_to_do_launches_nothing():
+    """No entries forward, neither gradient wanted backward: fine without a GPU."""
+    lib = _capi.load()
+    assert lib.vr_lookup_forward(C.byref(_lookup(n=0, ids=None)), None, None) == 0
+    assert lib.vr_lookup_backward(C.byref(_lookup()), 1 << 20, 3, None, None, None, 0, None) == 0
+
+
+def test_rows_that_lie_apart_are_taken_as_they_are():
+    t = torch.zeros(6, 5, 4)
+    assert embedding._row_layout(t, 1, 20)[1] == 20
+    part = t[:, 1:3]                                       # rows of 8 values, 20 apart
+    same, stride = embedding._row_layout(part, 1, 8)
+    assert same is part and stride == 20
+    for other in (t[:, :, 1:], t.transpose(0, 1), t[:1].expand(6, 5, 4), t[:, ::2]):
+        copy, stride = embedding._row_layout(other, 1, other[0].numel())
+        assert copy.is_contiguous() and stride == other[0].numel()
+    copy, stride = embedding._row_layout(part, 2, 4)       # two leading dimensions: not one stride
+    assert copy.is_contiguous() and stride == 4

@@ -33,6 +33,7 @@ EXPORTS = ["vr_abi_version", "vr_last_error", "vr_forward", "vr_backward", "vr_b
            "vr_densify_plan_words", "vr_densify_plan", "vr_densify_apply", "vr_reset_opacity",
            "vr_sh_grad_from_factors", "vr_sh_adam_step",
            "vr_grad_norm_scratch_bytes", "vr_grad_norm", "vr_clip_grads", "vr_clip_grad_norm", "vr_adam_step_clipped", "vr_sh_adam_step_clipped",
+           "vr_lookup_forward", "vr_lookup_scratch_bytes", "vr_lookup_backward",
            "vr_instances_forward", "vr_instances_backward", "vr_activations_forward", "vr_activations_backward",
            "vr_boxmodel_forward", "vr_boxmodel_backward", "vr_boxmodel_regularizer_grad",
            "vr_xgmi_create", "vr_xgmi_detach", "vr_xgmi_destroy", "vr_xgmi_layout", "vr_xgmi_window", "vr_xgmi_handle", "vr_xgmi_attach",
@@ -105,6 +106,12 @@ VR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # VrDat
 class VrShGradFactors(C.Structure):
     _fields_ = [("means3D", C.c_void_p), ("campos", C.c_void_p), ("factors", C.c_void_p), ("factor_view_stride", C.c_int64),
                 ("P", C.c_int32), ("n_views", C.c_int32), ("sh_degree", C.c_int32), ("scale", C.c_float)]
+
+
+class VrLookup(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("ids", C.c_void_p), ("row_scale", C.c_void_p), ("n", C.c_int64), ("rows", C.c_int64),
+                ("width", C.c_int64), ("table_stride", C.c_int64), ("table_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("ids_64", C.c_int32), ("scale", C.c_float)]
 
 
 class VrInstance(C.Structure):
@@ -240,6 +247,12 @@ def load():
     lib.vr_sh_adam_step_clipped.restype = C.c_int
     lib.vr_sh_adam_step_clipped.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
                                             C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
+    lib.vr_lookup_forward.restype = C.c_int
+    lib.vr_lookup_forward.argtypes = [C.POINTER(VrLookup), vp, vp]
+    lib.vr_lookup_scratch_bytes.restype = C.c_int64
+    lib.vr_lookup_scratch_bytes.argtypes = [C.c_int64] * 3
+    lib.vr_lookup_backward.restype = C.c_int
+    lib.vr_lookup_backward.argtypes = [C.POINTER(VrLookup), vp, C.c_int64, vp, vp, vp, C.c_int64, vp]
     lib.vr_instances_forward.restype = C.c_int
     lib.vr_instances_forward.argtypes = [C.POINTER(VrInstance), i32, vp, vp, vp, vp]
     lib.vr_instances_backward.restype = C.c_int

@@ -15,15 +15,16 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 LIB = os.path.join(OUT_DIR, "libvegsrast.so")
-SOURCES = ["api.hip", "preprocess.hip", "binning.hip", "render_fwd.hip", "render_bwd.hip", "preprocess_bwd.hip", "knn.hip", "losses.hip", "optim.hip", "instances.hip", "densify.hip", "xgmi.hip", "gradnorm.hip"]
-HEADERS = ["vr_device.h", "vr_host.h", "vr_segment.h", "vr_sh_factors.h", os.path.join("..", "..", "include", "vegs_rast.h"),
+SOURCES = ["api.hip", "preprocess.hip", "binning.hip", "render_fwd.hip", "render_bwd.hip", "preprocess_bwd.hip", "knn.hip", "losses.hip", "optim.hip", "instances.hip", "densify.hip", "xgmi.hip", "gradnorm.hip", "embedding.hip"]
+HEADERS = ["vr_device.h", "vr_host.h", "vr_segment.h", "vr_sh_factors.h", "vr_types.h", os.path.join("..", "..", "include", "vegs_rast.h"),
            os.path.join("..", "..", "include", "vegs_rast_debug.h"),
            os.path.join("..", "..", "include", "vegs_loss.h"), os.path.join("..", "..", "include", "vegs_optim.h"),
-           os.path.join("..", "..", "include", "vegs_instances.h"), os.path.join("..", "..", "include", "vegs_xgmi.h")]
+           os.path.join("..", "..", "include", "vegs_instances.h"), os.path.join("..", "..", "include", "vegs_xgmi.h"),
+           os.path.join("..", "..", "include", "vegs_embedding.h")]
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off", "-munsafe-fp-atomics", "-fPIC",
          "-fno-fast-math", "-Wall", "-Wno-unused-function"]
 # sources compiled without packed fp32 instructions (the two halves of a pair gain nothing where memory is the bound)
-NO_PACKED_FP32 = {"optim.hip", "gradnorm.hip"}
+NO_PACKED_FP32 = {"optim.hip", "gradnorm.hip", "embedding.hip"}
 NO_PACKED_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

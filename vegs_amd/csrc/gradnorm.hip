@@ -10,9 +10,7 @@
 #include "../../include/vegs_optim.h"
 #include "vr_host.h"
 #include "vr_sh_factors.h"
-
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+#include "vr_types.h"
 
 namespace vr {
 
@@ -33,22 +31,16 @@ struct GradArgs {
 
 __device__ __forceinline__ float grad_value(const void* p, long i, int dtype)
 {
-    if (dtype == VR_F32) return reinterpret_cast<const float*>(p)[i];
-    if (dtype == VR_BF16) return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
-    return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ uint16_t to_bf16(float x)       // nearest, ties to even; NaN stays NaN
-{
-    const uint32_t u = __float_as_uint(x);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+    if (dtype == VR_F32) return load_f32(reinterpret_cast<const float*>(p) + i);
+    if (dtype == VR_BF16) return load_f32(reinterpret_cast<const bf16*>(p) + i);
+    return load_f32(reinterpret_cast<const __half*>(p) + i);
 }
 __device__ __forceinline__ void grad_scale(void* p, long i, int dtype, float c)
 {
     const float x = c * grad_value(p, i, dtype);
-    if (dtype == VR_F32) reinterpret_cast<float*>(p)[i] = x;
-    else if (dtype == VR_BF16) reinterpret_cast<uint16_t*>(p)[i] = to_bf16(x);
-    else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+    if (dtype == VR_F32) store_f32(reinterpret_cast<float*>(p) + i, x);
+    else if (dtype == VR_BF16) store_f32(reinterpret_cast<bf16*>(p) + i, x);
+    else store_f32(reinterpret_cast<__half*>(p) + i, x);
 }
 
 // the norm's accumulator: a sum of squares, or the largest magnitude (a NaN, once met, stays)

@@ -1,0 +1,128 @@
+"""Rows of a shared, learnable table by index, scaled, with the gradients of the table and of the scales -- one launch forward
+(vegs_amd/csrc/embedding.hip, C ABI include/vegs_embedding.h).
+
+  lookup(table, ids, scale)     out[i] = scale[i] * table[ids[i]]
+
+What a model shares between its Gaussians, frames or instances is held once and looked up: an SH codebook (table [K, 15, 3],
+one id per Gaussian; the result IS the f_rest input of the rasterizer, next to instances.activate's outputs), per-image codes,
+pose corrections by frame.  The table's gradient is dense, in the table's type, so vegs_amd.optim.Adam, grad_norm and the
+exchanges of vegs_amd.dist take it like any other.  GPU tensors only; there is no CPU path.
+"""
+import ctypes as C
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+
+
+def _row_layout(t, lead, width):
+    """(t or a contiguous copy, elements between rows): `t` [*lead, ...] as rows of `width` contiguous elements."""
+    if t.is_contiguous():
+        return t, width
+    if lead == 1 and t.stride(0) >= width:
+        expect = 1
+        for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if n != 1 and st != expect:
+                return t.contiguous(), width
+            expect *= n
+        return t, t.stride(0)
+    return t.contiguous(), width
+
+
+def _arguments(table, ids, scale, width, out_dtype):
+    """(VrLookup, what has to stay alive)"""
+    table, stride = _row_layout(table, 1, width)
+    ids = ids.contiguous()
+    by_row = isinstance(scale, torch.Tensor)
+    s = scale.contiguous() if by_row else None
+    return _capi.VrLookup(_capi.ptr(table), _capi.ptr(ids), _capi.ptr(s), ids.numel(), table.shape[0], width, stride,
+                          _capi.VR_DTYPES[table.dtype], _capi.VR_DTYPES[out_dtype], int(ids.dtype == torch.int64),
+                          1.0 if by_row else scale), (table, ids, s)
+
+
+def _forward(table, ids, scale, width, dtype):
+    device = table.device
+    with torch.cuda.device(device):
+        out = torch.empty(ids.shape + table.shape[1:], dtype=dtype, device=device)
+        if out.numel():
+            lookup, keep = _arguments(table, ids, scale, width, dtype)
+            _capi.check(_capi.load().vr_lookup_forward(C.byref(lookup), out.data_ptr(),
+                                                       torch.cuda.current_stream(device).cuda_stream))
+    return out
+
+
+class _Lookup(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, table, ids, scale, width, dtype):
+        out = _forward(table, ids, scale, width, dtype)
+        ctx.scale, ctx.width, ctx.dtype = None if isinstance(scale, torch.Tensor) else scale, width, dtype
+        ctx.like = table.shape, table.dtype, table.device
+        # (the table's values are only needed for the gradient of the scales)
+        ctx.save_for_backward(table if ctx.needs_input_grad[2] else None, ids, scale if ctx.scale is None else None)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        table, ids, scale = ctx.saved_tensors
+        shape, dtype, device = ctx.like
+        width = ctx.width
+        want_table, want_scale = ctx.needs_input_grad[0], ctx.needs_input_grad[2]
+        with torch.cuda.device(device):
+            d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
+            d_scale = torch.empty(ids.shape, dtype=torch.float32, device=device) if want_scale else None
+            if width == 0 or ids.numel() == 0:
+                return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
+            g, g_stride = _row_layout(g, ids.dim(), width)
+            if table is None:                     # (a stand-in with the table's sizes: no value of it is read)
+                table = d_table
+            lookup, keep = _arguments(table, ids, ctx.scale if scale is None else scale, width, ctx.dtype)
+            lib = _capi.load()
+            scratch, nbytes = None, 0
+            if want_table:
+                nbytes = lib.vr_lookup_scratch_bytes(ids.numel(), shape[0], width)
+                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _capi.check(lib.vr_lookup_backward(C.byref(lookup), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
+                                               _capi.ptr(scratch), nbytes, torch.cuda.current_stream(device).cuda_stream))
+        return d_table, None, d_scale, None, None
+
+
+def lookup(table, ids, scale=None, dtype=None):
+    """scale * table[ids]: [*ids.shape, *table.shape[1:]], differentiable with respect to `table` and to a `scale` tensor.
+
+    table: [K, ...] float32, bfloat16 or float16.  ids: int32 or int64 of any shape; an id outside [0, K) -- -1 by
+    convention -- means "no row": zeros, and no gradient whatever stands in its place.  scale: a number, or a float32
+    tensor shaped like ids.  dtype: of the result, the table's (default) or float32.
+
+    The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in their order, in
+    float32, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same bits every time."""
+    if not isinstance(table, torch.Tensor) or not table.is_cuda:
+        raise ValueError("table must be a GPU tensor (there is no CPU path)")
+    if table.dim() < 1 or table.dtype not in _capi.VR_DTYPES or table.layout != torch.strided:
+        raise ValueError(f"table must be a dense float32, bfloat16 or float16 tensor [K, ...] (got {table.dtype} {tuple(table.shape)})")
+    device = table.device
+    if not isinstance(ids, torch.Tensor) or ids.device != device or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be an int32 or int64 tensor on {device}")
+    if ids.numel() >= 1 << 30 or table.shape[0] >= (1 << 31) - 1:
+        raise ValueError("at most 2^30 - 1 ids and 2^31 - 2 rows")
+    if scale is None:
+        scale = 1.0
+    if isinstance(scale, torch.Tensor):
+        if scale.device != device or scale.dtype != torch.float32 or scale.shape != ids.shape:
+            raise ValueError(f"a scale tensor must be float32 {tuple(ids.shape)} on {device}, shaped like ids "
+                             f"(got {scale.dtype} {tuple(scale.shape)} on {scale.device})")
+    else:
+        scale = float(scale)
+    if dtype is None:
+        dtype = table.dtype
+    elif dtype != table.dtype and dtype != torch.float32:
+        raise ValueError(f"the result has the table's type or float32 (got {dtype} for a table of {table.dtype})")
+    width = math.prod(table.shape[1:])
+    if width > 1 << 24:
+        raise ValueError("rows of more than 2^24 values")
+    if torch.is_grad_enabled() and (table.requires_grad or (isinstance(scale, torch.Tensor) and scale.requires_grad)):
+        return _Lookup.apply(table, ids, scale, width, dtype)
+    return _forward(table, ids, scale, width, dtype)
