@@ -14,6 +14,21 @@ struct LookupArgs {
     float scale;
 };
 
+// V values that lie next to each other, at any address their type may have: one load or store of up to 16 bytes
+template <typename T, int V>
+struct __attribute__((packed)) Pack { T v[V]; };
+
+__device__ __forceinline__ void zero_fill(char* p, long bytes, long at, long step)
+{
+    if (((uintptr_t)p & 15) == 0) {
+        const long n = bytes >> 4;
+        for (long i = at; i < n; i += step) nt_store4(make_float4(0.f, 0.f, 0.f, 0.f), reinterpret_cast<float4*>(p) + i);
+        for (long i = (n << 4) + 2 * at; i < bytes; i += 2 * step) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    } else {
+        for (long i = 2 * at; i < bytes; i += 2 * step) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    }
+}
+
 // the row of entry i, or -1
 __device__ __forceinline__ long row_of(const LookupArgs& a, long i)
 {
@@ -37,59 +52,257 @@ __global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict
     store_f32(out + e, x);
 }
 
-// sort keys: the row, or `rows` for "no row" (sorted behind every row); values: the entry
-__global__ void __launch_bounds__(256) k_lookup_keys(LookupArgs a, uint32_t* __restrict__ key, uint32_t* __restrict__ val)
+// First launch of the table's gradient: the sort's keys -- the row, or `rows` for "no row" (sorted behind every row) -- and its values,
+// the entries; workgroups behind those clear the gradient, of which only the rows with entries are written later.
+__global__ void __launch_bounds__(256)
+k_lookup_keys(LookupArgs a, uint32_t* __restrict__ key, uint32_t* __restrict__ val, int key_blocks, char* __restrict__ zero,
+              long zero_bytes)
 {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if ((int)blockIdx.x < key_blocks) {
+        const long i = (long)blockIdx.x * 256 + threadIdx.x;
+        if (i >= a.n) return;
+        const long row = row_of(a, i);
+        key[i] = row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
+        val[i] = (uint32_t)i;
+        return;
+    }
+    zero_fill(zero, zero_bytes, (long)(blockIdx.x - key_blocks) * 256 + threadIdx.x, (long)(gridDim.x - key_blocks) * 256);
+}
+
+// ---- the sums of the table's gradient over the sorted entries.
+//
+// Split by ENTRIES, not by rows, so that a row hit a million times costs what a million rows hit once do: a group of G lanes
+// (V columns each; G x V covers the width, or a tile of it) takes a chunk of consecutive sorted entries, keeps the running sum of the
+// current row in registers and stores it where the row changes.  A row that begins and ends inside the chunk goes straight to the
+// gradient; the sum of one that crosses the chunk's border goes to a slot of its own -- head: of the row that came in from the chunk
+// before; tail: of the row that begins here and goes on -- and k_lookup_join adds a row's tail and the heads behind it in order.
+// No atomics, and every order fixed by n and width alone.
+//
+// The gradient rows are gathered: each is one contiguous read of width x 4 bytes, UNROLL of them in flight per lane.
+constexpr int UNROLL = 8;
+constexpr uint32_t NO_ENTRY = 0xffffffffu;
+
+struct SumArgs {
+    const uint32_t *key, *val;
+    const void* grad;
+    long grad_stride;
+    void* d_table;
+    float* d_row_scale;
+    float* slots;                 // [chunks][2][width]: head, tail
+    int chunk;                    // entries of a chunk, a multiple of UNROLL
+    int g_shift;                  // G = 1 << g_shift lanes
+};
+
+template <typename TT, int V>
+__device__ __forceinline__ void store_row(TT* p, const float (&x)[V])
+{
+    Pack<TT, V> out;
+#pragma unroll
+    for (int v = 0; v < V; ++v) store_f32(out.v + v, x[v]);
+    *reinterpret_cast<Pack<TT, V>*>(p) = out;
+}
+
+template <typename TT, typename TO, int V, bool DSCALE>
+__global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
+{
+    const int G = 1 << q.g_shift, lane = threadIdx.x & (G - 1);
+    const long chunk = ((long)blockIdx.x * 256 + threadIdx.x) >> q.g_shift;
+    const long first = chunk * q.chunk, last = first + q.chunk < a.n ? first + q.chunk : a.n;
+    // the last lane of a row that is no multiple of V starts early and computes some of its neighbour's columns again
+    const long want = ((long)blockIdx.y * G + lane) * V;
+    const bool live = first < a.n && want < a.width;
+    const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
+    if (first >= a.n) return;               // (whole groups: the shuffles below stay inside a group)
+    const uint32_t rows = (uint32_t)a.rows;
+    const TO* grad = reinterpret_cast<const TO*>(q.grad) + col;
+    const TT* table = reinterpret_cast<const TT*>(a.table) + col;
+    TT* d_table = reinterpret_cast<TT*>(q.d_table) + col;
+    float* slot = q.slots + (2 * chunk) * a.width + col;
+    uint32_t cur = q.key[first];
+    bool came_in = first > 0 && q.key[first - 1] == cur;
+    float acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+    for (long j = first; j < last; j += UNROLL) {
+        uint32_t key[UNROLL], val[UNROLL];
+#pragma unroll
+        for (int x = 0; x < UNROLL; ++x) {
+            const bool in = j + x < last;
+            key[x] = in ? q.key[j + x] : NO_ENTRY;
+            val[x] = in ? q.val[j + x] : 0u;
+        }
+        Pack<TO, V> g[UNROLL];
+        Pack<TT, V> t[UNROLL];
+        float s[UNROLL];
+#pragma unroll
+        for (int x = 0; x < UNROLL; ++x) {
+            const bool there = key[x] < rows;
+            s[x] = there && a.row_scale ? a.row_scale[val[x]] : 1.0f;
+            g[x] = *reinterpret_cast<const Pack<TO, V>*>(grad + (there ? (long)val[x] * q.grad_stride : 0));
+            if (DSCALE) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (there ? (long)key[x] * a.table_stride : 0));
+        }
+        float dot[UNROLL];
+#pragma unroll
+        for (int x = 0; x < UNROLL; ++x) {
+            if (key[x] != cur && key[x] != NO_ENTRY) {
+                if (live && cur < rows) {
+                    if (came_in) store_row<float, V>(slot, acc);
+                    else store_row<TT, V>(d_table + (long)cur * a.width, acc);
+                }
+                came_in = false;
+                cur = key[x];
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+            }
+            dot[x] = 0.0f;
+            if (key[x] < rows) {
+                const float sx = a.scale * s[x];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float gv = load_f32(g[x].v + v);
+                    acc[v] = fmaf(sx, gv, acc[v]);
+                    if (DSCALE && col + v >= want) dot[x] = fmaf(gv, load_f32(t[x].v + v), dot[x]);
+                }
+            }
+        }
+        if (DSCALE) {
+#pragma unroll
+            for (int x = 0; x < UNROLL; ++x) {
+                float d = live ? dot[x] : 0.0f;
+                for (int w = G >> 1; w > 0; w >>= 1) d += __shfl_xor(d, w, 64);
+                if (lane == 0 && j + x < last) q.d_row_scale[val[x]] = a.scale * d;
+            }
+        }
+    }
+    if (live && cur < rows) {
+        const bool goes_on = last < a.n && q.key[last] == cur;
+        if (came_in) store_row<float, V>(slot, acc);
+        else if (goes_on) store_row<float, V>(slot + a.width, acc);
+        else store_row<TT, V>(d_table + (long)cur * a.width, acc);
+    }
+}
+
+// Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at JOIN_CHUNKS chunks; short
+// rows are one group's each, rows of more than JOIN_LONG pieces the whole workgroup's: group k adds the pieces k, k + groups, ... and
+// the groups' sums are added in order.
+constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 32;
+
+template <typename TT, int V>
+__global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumArgs q, long chunks)
+{
+    __shared__ long from[JOIN_CHUNKS], upto[JOIN_CHUNKS];
+    __shared__ uint32_t row[JOIN_CHUNKS];
+    __shared__ int count;
+    __shared__ float part[JOIN_THREADS * V];
+    const int G = 1 << q.g_shift, lane = threadIdx.x & (G - 1), group = threadIdx.x >> q.g_shift, groups = JOIN_THREADS >> q.g_shift;
+    const long want = ((long)blockIdx.y * G + lane) * V;
+    const bool live = want < a.width;
+    const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
+    if (threadIdx.x < JOIN_CHUNKS) {
+        const long c = (long)blockIdx.x * JOIN_CHUNKS + threadIdx.x, first = c * q.chunk, next = first + q.chunk;
+        bool owner = false;
+        uint32_t k = 0;
+        if (c < chunks && next < a.n) {
+            k = q.key[next - 1];
+            // its last row goes on, and begins in this chunk
+            owner = k < (uint32_t)a.rows && q.key[next] == k && (first == 0 || q.key[first - 1] != k);
+        }
+        const unsigned long long mask = __ballot(owner);           // (one wave: JOIN_CHUNKS is 64)
+        if (threadIdx.x == 0) count = __popcll(mask);
+        if (owner) {
+            // the last chunk whose first entry is of this row: doubling steps, then halving ones
+            long lo = c + 1, step = 1;
+            while (lo + step < chunks && q.key[(lo + step) * q.chunk] == k) { lo += step; step <<= 1; }
+            for (; step > 0; step >>= 1)
+                if (lo + step < chunks && q.key[(lo + step) * q.chunk] == k) lo += step;
+            const int at = __popcll(mask & ((1ull << threadIdx.x) - 1ull));
+            from[at] = c; upto[at] = lo; row[at] = k;
+        }
+    }
+    __syncthreads();
+    const float* slots = q.slots + col;
+    TT* d_table = reinterpret_cast<TT*>(q.d_table) + col;
+    for (int o = group; o < count; o += groups) {
+        const long c = from[o], end = upto[o];
+        if (end - c > JOIN_LONG || !live) continue;
+        Pack<float, V> acc = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * c + 1) * a.width);
+        for (long p = c + 1; p <= end; ++p) {
+            const Pack<float, V> h = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * p) * a.width);
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc.v[v] += h.v[v];
+        }
+        store_row<TT, V>(d_table + (long)row[o] * a.width, acc.v);
+    }
+    for (int o = 0; o < count; ++o) {
+        const long c = from[o], end = upto[o];
+        if (end - c <= JOIN_LONG) continue;                         // (the same for every thread)
+        float acc[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        for (long p = c + group; p <= end; p += groups) {           // piece c is the tail
+            const Pack<float, V> h = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * p + (p == c)) * a.width);
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] += h.v[v];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
+        __syncthreads();
+        if (group == 0 && live) {
+            for (int k = 1; k < groups; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += part[((k << q.g_shift) + lane) * V + v];
+            store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
+        }
+    }
+}
+
+// The scales' gradient alone, entry by entry: where the table's is not wanted, or the width takes more than one tile.
+template <typename TT, typename TO, int V>
+__global__ void __launch_bounds__(256) k_lookup_dscale(LookupArgs a, const TO* __restrict__ grad, long grad_stride,
+                                                       float* __restrict__ d_row_scale, int g_shift)
+{
+    const int G = 1 << g_shift, lane = threadIdx.x & (G - 1);
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) >> g_shift;
     if (i >= a.n) return;
     const long row = row_of(a, i);
-    key[i] = row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
-    val[i] = (uint32_t)i;
-}
-
-__device__ __forceinline__ long lower_bound(const uint32_t* key, long n, uint32_t k)
-{
-    long lo = 0, hi = n;
-    while (lo < hi) {
-        const long mid = (lo + hi) >> 1;
-        if (key[mid] < k) lo = mid + 1; else hi = mid;
-    }
-    return lo;
-}
-
-// one wave per row of the table: the row's entries one after the other, lanes across the columns
-template <typename TT, typename TO>
-__global__ void __launch_bounds__(64)
-k_lookup_sum(LookupArgs a, const TO* __restrict__ grad, long grad_stride, const uint32_t* __restrict__ key,
-             const uint32_t* __restrict__ val, TT* __restrict__ d_table)
-{
-    const long row = blockIdx.x;
-    const long first = lower_bound(key, a.n, (uint32_t)row), last = lower_bound(key, a.n, (uint32_t)row + 1);
-    for (long c = threadIdx.x; c < a.width; c += 64) {
-        float acc = 0.0f;
-        for (long j = first; j < last; ++j) {
-            const long i = val[j];
-            const float s = a.row_scale ? a.scale * a.row_scale[i] : a.scale;
-            acc = fmaf(s, load_f32(grad + i * grad_stride + c), acc);
-        }
-        store_f32(d_table + row * a.width + c, acc);
-    }
-}
-
-// one wave per entry
-template <typename TT, typename TO>
-__global__ void __launch_bounds__(64)
-k_lookup_dscale(LookupArgs a, const TO* __restrict__ grad, long grad_stride, float* __restrict__ d_row_scale)
-{
-    const long i = blockIdx.x, row = row_of(a, i);
     float acc = 0.0f;
-    if (row >= 0)
-        for (long c = threadIdx.x; c < a.width; c += 64)
-            acc = fmaf(load_f32(grad + i * grad_stride + c),
-                       load_f32(reinterpret_cast<const TT*>(a.table) + row * a.table_stride + c), acc);
+    if (row >= 0) {
+        const TO* g = grad + i * grad_stride;
+        const TT* t = reinterpret_cast<const TT*>(a.table) + row * a.table_stride;
+        for (long want = (long)lane * V; want < a.width; want += G * V) {
+            const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
+            const Pack<TO, V> x = *reinterpret_cast<const Pack<TO, V>*>(g + col);
+            const Pack<TT, V> y = *reinterpret_cast<const Pack<TT, V>*>(t + col);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) acc += __shfl_xor(acc, d, 64);
-    if (threadIdx.x == 0) d_row_scale[i] = a.scale * acc;
+            for (int v = 0; v < V; ++v)
+                if (col + v >= want) acc = fmaf(load_f32(x.v + v), load_f32(y.v + v), acc);
+        }
+    }
+    for (int w = G >> 1; w > 0; w >>= 1) acc += __shfl_xor(acc, w, 64);
+    if (lane == 0) d_row_scale[i] = a.scale * acc;
+}
+
+// Lanes and columns for a width: V values (16 bytes of the result's type) per lane, or one where the row is shorter than that.
+struct Tiling {
+    int V, g_shift, tiles, chunk;
+    long chunks;
+};
+static Tiling tiling(int64_t n, int64_t width, int v_full)
+{
+    Tiling t;
+    t.V = width >= v_full ? v_full : 1;
+    const int64_t lanes = (width + t.V - 1) / t.V;
+    t.g_shift = 0;
+    while (t.g_shift < 6 && (1 << t.g_shift) < lanes) ++t.g_shift;
+    t.tiles = (int)((lanes + 63) / 64);
+    // long chunks make few slots; shorter ones while there are fewer than four waves for each of the 1024 SIMDs -- but no more than
+    // 8192 of them, which is what one workgroup has to join where all entries are of one row (at 16384 entries of 1024 16-bit
+    // values: 13 us with four waves per SIMD, 19 with one)
+    t.chunk = 64;
+    while (t.chunk > UNROLL && ((n << t.g_shift) / 64 / t.chunk) * t.tiles < 4096 && n <= 4096l * t.chunk) t.chunk >>= 1;
+    t.chunks = (long)((n + t.chunk - 1) / t.chunk);
+    return t;
 }
 
 static int check_lookup(const VrLookup* l, LookupArgs& a)
@@ -137,17 +350,33 @@ struct Forward {
     }
 };
 
+// Everything after the sort.
 struct Backward {
-    template <typename TT, typename TO>
-    static int run(const LookupArgs& a, const void* grad, long grad_stride, const uint32_t* key, const uint32_t* val, void* d_table,
-                   float* d_row_scale, hipStream_t s)
+    template <typename TT, typename TO, int V>
+    static void launch(const LookupArgs& a, const SumArgs& q, const Tiling& t, hipStream_t s)
     {
-        if (d_table && a.rows > 0)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO>), dim3((unsigned)a.rows), dim3(64), 0, s, a, (const TO*)grad,
-                               grad_stride, key, val, (TT*)d_table);
-        if (d_row_scale && a.n > 0)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_dscale<TT, TO>), dim3((unsigned)a.n), dim3(64), 0, s, a, (const TO*)grad,
-                               grad_stride, d_row_scale);
+        const bool fused = q.d_row_scale && q.d_table && t.tiles == 1;
+        if (q.d_table) {
+            const dim3 grid((unsigned)(((t.chunks << t.g_shift) + 255) / 256), t.tiles);
+            if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, true>), grid, dim3(256), 0, s, a, q);
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, false>), grid, dim3(256), 0, s, a, q);
+            if (t.chunks > 1)
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_join<TT, V>), dim3((unsigned)((t.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS), t.tiles),
+                                   dim3(JOIN_THREADS), 0, s, a, q, t.chunks);
+        }
+        if (q.d_row_scale && !fused)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_dscale<TT, TO, V>), dim3((unsigned)(((a.n << t.g_shift) + 255) / 256)), dim3(256),
+                               0, s, a, reinterpret_cast<const TO*>(q.grad), q.grad_stride, q.d_row_scale, t.g_shift);
+    }
+    template <typename TT, typename TO>
+    static int run(const LookupArgs& a, SumArgs q, hipStream_t s)
+    {
+        constexpr int V = 16 / sizeof(TO);
+        const Tiling t = tiling(a.n, a.width, V);
+        q.chunk = t.chunk;
+        q.g_shift = t.g_shift;
+        if (t.V == V) launch<TT, TO, V>(a, q, t, s);
+        else launch<TT, TO, 1>(a, q, t, s);
         if (hipGetLastError() != hipSuccess) { set_error("lookup: kernel launch failed"); return VR_ERR_HIP; }
         return VR_OK;
     }
@@ -167,10 +396,19 @@ extern "C" int vr_lookup_forward(const VrLookup* lookup, void* out, void* stream
     return by_type<Forward>(lookup, a, out, (hipStream_t)stream);
 }
 
+// scratch: two pairs of key and value arrays, the sort's own, and the slots of the chunks (a chunk has UNROLL entries at
+// least; the tiling of the wider type has the shorter chunks)
+static size_t slots_bytes(int64_t n, int64_t width)
+{
+    const long chunks = tiling(n, width, 4).chunks > tiling(n, width, 8).chunks ? tiling(n, width, 4).chunks : tiling(n, width, 8).chunks;
+    return align_up((size_t)chunks * 2 * (size_t)width * sizeof(float), 256);
+}
+
 extern "C" int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width)
 {
     if (n < 0 || n >= (1ll << 30) || rows < 0 || rows >= 0x7fffffffll || width < 1 || width > (1 << 24)) return 0;
-    return (int64_t)(4 * align_up((size_t)(n > 0 ? n : 1) * 4, 256) + sort_pairs_scratch_bytes((long)n));
+    if (n == 0) n = 1;
+    return (int64_t)(4 * align_up((size_t)n * 4, 256) + align_up(sort_pairs_scratch_bytes((long)n), 256) + slots_bytes(n, width));
 }
 
 extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int64_t grad_stride, void* d_table, float* d_row_scale,
@@ -184,19 +422,25 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
         { set_error("lookup: grad is required, arrays aligned to their elements, grad_stride >= width"); return VR_ERR_INVALID_ARGUMENT; }
     if (d_table && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < vr_lookup_scratch_bytes(a.n, a.rows, a.width)))
         { set_error("lookup: the table's gradient needs vr_lookup_scratch_bytes of scratch, 256-byte aligned"); return VR_ERR_INVALID_ARGUMENT; }
-    if ((!d_table || a.rows == 0) && (!d_row_scale || a.n == 0)) return VR_OK;
+    if (a.rows == 0) d_table = nullptr;
+    if (!d_table && (!d_row_scale || a.n == 0)) return VR_OK;
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t *key = nullptr, *val = nullptr;
-    if (d_table && a.n > 0) {
-        const size_t arr = align_up((size_t)a.n * 4, 256);
+    SumArgs q{nullptr, nullptr, grad, (long)grad_stride, d_table, d_row_scale, nullptr, 0, 0};
+    if (d_table) {
+        const size_t arr = align_up((size_t)(a.n > 0 ? a.n : 1) * 4, 256);
         char* base = (char*)scratch;
         uint32_t *k0 = (uint32_t*)base, *v0 = (uint32_t*)(base + arr), *k1 = (uint32_t*)(base + 2 * arr), *v1 = (uint32_t*)(base + 3 * arr);
-        hipLaunchKernelGGL(k_lookup_keys, dim3(cdiv(a.n, 256)), dim3(256), 0, s, a, k0, v0);
+        const long zero_bytes = a.rows * a.width * (long)t_element, zero_blocks = (zero_bytes + 16383) / 16384;
+        const int key_blocks = cdiv(a.n, 256);
+        hipLaunchKernelGGL(k_lookup_keys, dim3(key_blocks + (unsigned)(zero_blocks < 4096 ? zero_blocks : 4096)), dim3(256), 0, s, a, k0, v0,
+                           key_blocks, (char*)d_table, zero_bytes);
         VR_KERNEL_CHECK("lookup_keys", s, false);
+        if (a.n == 0) return VR_OK;
         int where = 0;
         if (int rc = launch_sort_pairs(k0, v0, k1, v1, a.n, 0u, key_bits(a.rows), base + 4 * arr, s, false, &where)) return rc;
-        key = where ? k1 : k0;
-        val = where ? v1 : v0;
+        q.key = where ? k1 : k0;
+        q.val = where ? v1 : v0;
+        q.slots = (float*)(base + 4 * arr + align_up(sort_pairs_scratch_bytes(a.n), 256));
     }
-    return by_type<Backward>(lookup, a, grad, (long)grad_stride, key, val, d_table, d_row_scale, s);
+    return by_type<Backward>(lookup, a, q, s);
 }
