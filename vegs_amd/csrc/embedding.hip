@@ -3,6 +3,8 @@
 #include "vr_host.h"
 #include "vr_types.h"
 
+#include <type_traits>
+
 namespace vr {
 
 struct LookupArgs {
@@ -17,6 +19,37 @@ struct LookupArgs {
 // V values that lie next to each other, at any address their type may have: one load or store of up to 16 bytes
 template <typename T, int V>
 struct __attribute__((packed)) Pack { T v[V]; };
+
+// 16 bytes at an address of 2 or 4 bytes' alignment, past the caches' normal order of replacement
+typedef uint32_t quad_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t quad_2 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_once(const T* p)
+{
+    if (sizeof(Pack<T, V>) != 16) return *reinterpret_cast<const Pack<T, V>*>(p);
+    using Q = typename std::conditional<sizeof(T) == 4, quad_4, quad_2>::type;
+    const Q q = __builtin_nontemporal_load(reinterpret_cast<const Q*>(p));
+    Pack<T, V> out;
+    __builtin_memcpy(&out, &q, sizeof(out) < 16 ? sizeof(out) : 16);
+    return out;
+}
+
+template <typename TT, int V, bool NT = false>
+__device__ __forceinline__ void store_row(TT* p, const float (&x)[V])
+{
+    Pack<TT, V> out;
+#pragma unroll
+    for (int v = 0; v < V; ++v) store_f32(out.v + v, x[v]);
+    if (NT && sizeof(out) == 16) {
+        using Q = typename std::conditional<sizeof(TT) == 4, quad_4, quad_2>::type;
+        Q q;
+        __builtin_memcpy(&q, &out, sizeof(out) < 16 ? sizeof(out) : 16);
+        __builtin_nontemporal_store(q, reinterpret_cast<Q*>(p));
+    } else {
+        *reinterpret_cast<Pack<TT, V>*>(p) = out;
+    }
+}
 
 __device__ __forceinline__ void zero_fill(char* p, long bytes, long at, long step)
 {
@@ -36,20 +69,46 @@ __device__ __forceinline__ long row_of(const LookupArgs& a, long i)
     return id >= 0 && id < a.rows ? id : -1;
 }
 
-template <typename TT, typename TO>
-__global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict__ out)
+// A group of G lanes per entry, V columns (16 bytes of the result) per lane; a wave takes 64 / G entries that follow one another at a
+// time, so that its stores are one contiguous piece, and FWD_ENTRIES of them, so that as many gathers are in flight.
+// NT: stores past the caches' normal replacement, for results larger than all L2s together: rows of 180 bytes begin and end inside a
+// line, and lines that wait in the L2 for their other part crowd out what is being gathered (2 M rows of 45 floats: 121 us without,
+// 67 with, 5.6 TB/s).  Smaller results are left in the caches for who reads them next.
+constexpr int FWD_ENTRIES = 4;
+constexpr long FWD_NT_BYTES = 32l << 20;
+
+template <typename TT, typename TO, int V, bool NT>
+__global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict__ out, int g_shift)
 {
-    const long e = (long)blockIdx.x * 256 + threadIdx.x;
-    if (e >= a.n * a.width) return;
-    const long i = e / a.width, c = e - i * a.width;
-    const long row = row_of(a, i);
-    float x = 0.0f;
-    if (row >= 0) {
-        x = load_f32(reinterpret_cast<const TT*>(a.table) + row * a.table_stride + c);
-        if (a.row_scale) x *= a.scale * a.row_scale[i];
-        else x *= a.scale;
+    const int G = 1 << g_shift, lane = threadIdx.x & (G - 1), per = 64 >> g_shift;
+    const long want = ((long)blockIdx.y * G + lane) * V;
+    if (want >= a.width) return;
+    // the last lane of a row that is no multiple of V starts early and writes some of its neighbour's columns again
+    const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
+    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long first = wave * (per * FWD_ENTRIES) + ((threadIdx.x & 63) >> g_shift);
+    const TT* table = reinterpret_cast<const TT*>(a.table) + col;
+    long row[FWD_ENTRIES];
+    float s[FWD_ENTRIES];
+#pragma unroll
+    for (int x = 0; x < FWD_ENTRIES; ++x) {
+        const long i = first + x * per;
+        row[x] = i < a.n ? row_of(a, i) : -1;
+        s[x] = i < a.n && a.row_scale ? a.row_scale[i] : 1.0f;
     }
-    store_f32(out + e, x);
+    Pack<TT, V> t[FWD_ENTRIES];
+#pragma unroll
+    for (int x = 0; x < FWD_ENTRIES; ++x)
+        if (row[x] >= 0) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + row[x] * a.table_stride);
+#pragma unroll
+    for (int x = 0; x < FWD_ENTRIES; ++x) {
+        const long i = first + x * per;
+        if (i >= a.n) return;
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[v] = row[x] >= 0 ? a.scale * s[x] * load_f32(t[x].v + v) : 0.0f;
+        store_row<TO, V, NT>(out + i * a.width + col, y);
+    }
 }
 
 // First launch of the table's gradient: the sort's keys -- the row, or `rows` for "no row" (sorted behind every row) -- and its values,
@@ -93,15 +152,6 @@ struct SumArgs {
     int g_shift;                  // G = 1 << g_shift lanes
 };
 
-template <typename TT, int V>
-__device__ __forceinline__ void store_row(TT* p, const float (&x)[V])
-{
-    Pack<TT, V> out;
-#pragma unroll
-    for (int v = 0; v < V; ++v) store_f32(out.v + v, x[v]);
-    *reinterpret_cast<Pack<TT, V>*>(p) = out;
-}
-
 template <typename TT, typename TO, int V, bool DSCALE>
 __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 {
@@ -118,6 +168,13 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
     const TT* table = reinterpret_cast<const TT*>(a.table) + col;
     TT* d_table = reinterpret_cast<TT*>(q.d_table) + col;
     float* slot = q.slots + (2 * chunk) * a.width + col;
+    // (the arrays are padded to whole chunks: the loads of keys and entries need no bounds, what lies behind `last` is masked)
+    uint4 next_key[UNROLL / 4], next_val[UNROLL / 4];
+#pragma unroll
+    for (int x = 0; x < UNROLL / 4; ++x) {
+        next_key[x] = reinterpret_cast<const uint4*>(q.key + first)[x];
+        next_val[x] = reinterpret_cast<const uint4*>(q.val + first)[x];
+    }
     uint32_t cur = q.key[first];
     bool came_in = first > 0 && q.key[first - 1] == cur;
     float acc[V];
@@ -128,8 +185,8 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 #pragma unroll
         for (int x = 0; x < UNROLL; ++x) {
             const bool in = j + x < last;
-            key[x] = in ? q.key[j + x] : NO_ENTRY;
-            val[x] = in ? q.val[j + x] : 0u;
+            key[x] = in ? (&next_key[x / 4].x)[x % 4] : NO_ENTRY;
+            val[x] = in ? (&next_val[x / 4].x)[x % 4] : 0u;
         }
         Pack<TO, V> g[UNROLL];
         Pack<TT, V> t[UNROLL];
@@ -138,8 +195,15 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
         for (int x = 0; x < UNROLL; ++x) {
             const bool there = key[x] < rows;
             s[x] = there && a.row_scale ? a.row_scale[val[x]] : 1.0f;
-            g[x] = *reinterpret_cast<const Pack<TO, V>*>(grad + (there ? (long)val[x] * q.grad_stride : 0));
+            g[x] = load_once<TO, V>(grad + (there ? (long)val[x] * q.grad_stride : 0));
             if (DSCALE) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (there ? (long)key[x] * a.table_stride : 0));
+        }
+        if (j + UNROLL < last) {               // the next ones travel while these rows are added
+#pragma unroll
+            for (int x = 0; x < UNROLL / 4; ++x) {
+                next_key[x] = reinterpret_cast<const uint4*>(q.key + j + UNROLL)[x];
+                next_val[x] = reinterpret_cast<const uint4*>(q.val + j + UNROLL)[x];
+            }
         }
         float dot[UNROLL];
 #pragma unroll
@@ -185,7 +249,27 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 // Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at JOIN_CHUNKS chunks; short
 // rows are one group's each, rows of more than JOIN_LONG pieces the whole workgroup's: group k adds the pieces k, k + groups, ... and
 // the groups' sums are added in order.
-constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 32;
+constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 16, JOIN_AHEAD = 8;
+
+// acc += the pieces p, p + step, ... up to `end` of the row whose tail is piece c, JOIN_AHEAD of them in flight
+template <int V>
+__device__ __forceinline__ void join_pieces(float (&acc)[V], const float* __restrict__ slots, long width, long c, long p, long end,
+                                            long step)
+{
+    for (; p <= end; p += JOIN_AHEAD * step) {
+        Pack<float, V> h[JOIN_AHEAD];
+#pragma unroll
+        for (int x = 0; x < JOIN_AHEAD; ++x) {
+            const long at = p + x * step <= end ? p + x * step : p;
+            h[x] = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * at + (at == c)) * width);
+        }
+#pragma unroll
+        for (int x = 0; x < JOIN_AHEAD; ++x)
+            if (p + x * step <= end)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += h[x].v[v];
+    }
+}
 
 template <typename TT, int V>
 __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumArgs q, long chunks)
@@ -225,13 +309,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
     for (int o = group; o < count; o += groups) {
         const long c = from[o], end = upto[o];
         if (end - c > JOIN_LONG || !live) continue;
-        Pack<float, V> acc = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * c + 1) * a.width);
-        for (long p = c + 1; p <= end; ++p) {
-            const Pack<float, V> h = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * p) * a.width);
+        float acc[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) acc.v[v] += h.v[v];
-        }
-        store_row<TT, V>(d_table + (long)row[o] * a.width, acc.v);
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        join_pieces<V>(acc, slots, a.width, c, c, end, 1);
+        store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
     }
     for (int o = 0; o < count; ++o) {
         const long c = from[o], end = upto[o];
@@ -239,11 +321,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        for (long p = c + group; p <= end; p += groups) {           // piece c is the tail
-            const Pack<float, V> h = *reinterpret_cast<const Pack<float, V>*>(slots + (2 * p + (p == c)) * a.width);
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] += h.v[v];
-        }
+        join_pieces<V>(acc, slots, a.width, c, c + group, end, groups);
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
@@ -342,9 +420,14 @@ struct Forward {
     template <typename TT, typename TO>
     static int run(const LookupArgs& a, void* out, hipStream_t s)
     {
-        const long blocks = (a.n * a.width + 255) / 256;
-        if (blocks > 0x7fffffffl) { set_error("lookup: n x width is too large"); return VR_ERR_INVALID_ARGUMENT; }
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO>), dim3((unsigned)blocks), dim3(256), 0, s, a, (TO*)out);
+        constexpr int V = 16 / sizeof(TO);
+        const Tiling t = tiling(a.n, a.width, V);
+        const long per = 4 * (64 >> t.g_shift) * FWD_ENTRIES;
+        const dim3 grid((unsigned)((a.n + per - 1) / per), t.tiles);
+        if (t.V != V) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO, 1, false>), grid, dim3(256), 0, s, a, (TO*)out, t.g_shift);
+        else if (a.n * a.width * (long)sizeof(TO) >= FWD_NT_BYTES)
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO, V, true>), grid, dim3(256), 0, s, a, (TO*)out, t.g_shift);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO, V, false>), grid, dim3(256), 0, s, a, (TO*)out, t.g_shift);
         if (hipGetLastError() != hipSuccess) { set_error("lookup: kernel launch failed"); return VR_ERR_HIP; }
         return VR_OK;
     }
