@@ -128,6 +128,94 @@ k_lookup_keys(LookupArgs a, uint32_t* __restrict__ key, uint32_t* __restrict__ v
     zero_fill(zero, zero_bytes, (long)(blockIdx.x - key_blocks) * 256 + threadIdx.x, (long)(gridDim.x - key_blocks) * 256);
 }
 
+// The same for up to SORT_SMALL entries, sorted as well: one workgroup holds them in LDS through all passes (stable, 8 bits each),
+// the others clear the gradient meanwhile.  One launch where the general sort takes a launch for the keys and four a pass: at
+// 16384 entries and 32000 rows 49 us of kernels, and as much again between them.
+constexpr int SORT_SMALL = 16384, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+
+template <int ITEMS>
+__global__ void __launch_bounds__(SORT_THREADS)
+k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict__ val_out, int bits, char* __restrict__ zero, long zero_bytes)
+{
+    __shared__ uint32_t cnt[SORT_WAVES][256], base[256], wave_sum[4];
+    __shared__ uint32_t skey[SORT_THREADS * ITEMS], sval[SORT_THREADS * ITEMS];
+    if (blockIdx.x > 0) {
+        zero_fill(zero, zero_bytes, (long)(blockIdx.x - 1) * SORT_THREADS + threadIdx.x, (long)(gridDim.x - 1) * SORT_THREADS);
+        return;
+    }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * ITEMS) + lane;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        const int i = first + 64 * x;
+        const long row = i < a.n ? row_of(a, i) : -1;
+        key[x] = i < a.n ? (row >= 0 ? (uint32_t)row : (uint32_t)a.rows) : 0xffffffffu;   // what is padding stays last
+        val[x] = (uint32_t)i;
+    }
+    for (int shift = 0; shift < bits; shift += 8) {
+        for (int d = threadIdx.x; d < SORT_WAVES * 256; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
+        __syncthreads();
+        // the entry's place among those of its digit in its wave: lanes of the same digit by ballots, earlier items from the count
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            const uint32_t d = (key[x] >> shift) & 255u;
+            unsigned long long same = ~0ull;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                const unsigned long long on = __ballot((d >> b) & 1u);
+                same &= ((d >> b) & 1u) ? on : ~on;
+            }
+            const uint32_t prior = cnt[w][d];
+            rank[x] = prior + (uint32_t)__popcll(same & before);
+            __builtin_amdgcn_wave_barrier();
+            if ((same & before) == 0) cnt[w][d] = prior + (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        // exclusive sums over (digit, wave)
+        uint32_t total = 0, incl = 0;
+        if (threadIdx.x < 256) {
+            for (int k = 0; k < SORT_WAVES; ++k) {
+                const uint32_t c = cnt[k][threadIdx.x];
+                cnt[k][threadIdx.x] = total;
+                total += c;
+            }
+            incl = total;
+#pragma unroll
+            for (int dd = 1; dd < 64; dd <<= 1) {
+                const uint32_t o = (uint32_t)__shfl_up((int)incl, dd, 64);
+                if (lane >= dd) incl += o;
+            }
+            if (lane == 63) wave_sum[w] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            uint32_t b = incl - total;
+            for (int k = 0; k < w; ++k) b += wave_sum[k];
+            base[threadIdx.x] = b;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            const uint32_t d = (key[x] >> shift) & 255u, at = base[d] + cnt[w][d] + rank[x];
+            skey[at] = key[x];
+            sval[at] = val[x];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            key[x] = skey[first + 64 * x];
+            val[x] = sval[first + 64 * x];
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        const int i = first + 64 * x;
+        if (i < a.n) { key_out[i] = key[x]; val_out[i] = val[x]; }
+    }
+}
+
 // ---- the sums of the table's gradient over the sorted entries.
 //
 // Split by ENTRIES, not by rows, so that a row hit a million times costs what a million rows hit once do: a group of G lanes
@@ -514,15 +602,26 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
         char* base = (char*)scratch;
         uint32_t *k0 = (uint32_t*)base, *v0 = (uint32_t*)(base + arr), *k1 = (uint32_t*)(base + 2 * arr), *v1 = (uint32_t*)(base + 3 * arr);
         const long zero_bytes = a.rows * a.width * (long)t_element, zero_blocks = (zero_bytes + 16383) / 16384;
-        const int key_blocks = cdiv(a.n, 256);
-        hipLaunchKernelGGL(k_lookup_keys, dim3(key_blocks + (unsigned)(zero_blocks < 4096 ? zero_blocks : 4096)), dim3(256), 0, s, a, k0, v0,
-                           key_blocks, (char*)d_table, zero_bytes);
-        VR_KERNEL_CHECK("lookup_keys", s, false);
-        if (a.n == 0) return VR_OK;
-        int where = 0;
-        if (int rc = launch_sort_pairs(k0, v0, k1, v1, a.n, 0u, key_bits(a.rows), base + 4 * arr, s, false, &where)) return rc;
-        q.key = where ? k1 : k0;
-        q.val = where ? v1 : v0;
+        if (a.n > 0 && a.n <= SORT_SMALL) {
+            const dim3 grid(1 + (unsigned)(zero_blocks < 1024 ? zero_blocks : 1024));
+            const int bits = key_bits(a.rows);
+            if (a.n <= SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<1>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
+            else if (a.n <= 4 * SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
+            else hipLaunchKernelGGL(k_lookup_sort<16>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
+            VR_KERNEL_CHECK("lookup_sort", s, false);
+            q.key = k0;
+            q.val = v0;
+        } else {
+            const int key_blocks = cdiv(a.n, 256);
+            hipLaunchKernelGGL(k_lookup_keys, dim3(key_blocks + (unsigned)(zero_blocks < 4096 ? zero_blocks : 4096)), dim3(256), 0, s, a, k0,
+                               v0, key_blocks, (char*)d_table, zero_bytes);
+            VR_KERNEL_CHECK("lookup_keys", s, false);
+            if (a.n == 0) return VR_OK;
+            int where = 0;
+            if (int rc = launch_sort_pairs(k0, v0, k1, v1, a.n, 0u, key_bits(a.rows), base + 4 * arr, s, false, &where)) return rc;
+            q.key = where ? k1 : k0;
+            q.val = where ? v1 : v0;
+        }
         q.slots = (float*)(base + 4 * arr + align_up(sort_pairs_scratch_bytes(a.n), 256));
     }
     return by_type<Backward>(lookup, a, q, s);

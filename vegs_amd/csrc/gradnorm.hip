@@ -29,19 +29,9 @@ struct GradArgs {
     int count, units;
 };
 
-__device__ __forceinline__ float grad_value(const void* p, long i, int dtype)
-{
-    if (dtype == VR_F32) return load_f32(reinterpret_cast<const float*>(p) + i);
-    if (dtype == VR_BF16) return load_f32(reinterpret_cast<const bf16*>(p) + i);
-    return load_f32(reinterpret_cast<const __half*>(p) + i);
-}
-__device__ __forceinline__ void grad_scale(void* p, long i, int dtype, float c)
-{
-    const float x = c * grad_value(p, i, dtype);
-    if (dtype == VR_F32) store_f32(reinterpret_cast<float*>(p) + i, x);
-    else if (dtype == VR_BF16) store_f32(reinterpret_cast<bf16*>(p) + i, x);
-    else store_f32(reinterpret_cast<__half*>(p) + i, x);
-}
+// 16 bytes of values at an address of their own alignment (a gradient may be a view that starts anywhere)
+template <typename T>
+struct __attribute__((packed)) Quad { T v[16 / sizeof(T)]; };
 
 // the norm's accumulator: a sum of squares, or the largest magnitude (a NaN, once met, stays)
 template <bool MAX>
@@ -81,18 +71,43 @@ __device__ __forceinline__ GradSeg grad_seg(const GradArgs& a, int unit)
     return a.seg[t];
 }
 
+// A unit's values: four loads of 16 bytes per thread at once where the unit is full, single values in a tensor's last unit.
+// Two accumulators, for the 64-bit multiply-add's latency.
+template <bool MAX, typename T>
+__device__ __forceinline__ void norm_unit(const void* data, long base, long n, double& acc0, double& acc1)
+{
+    constexpr int V = 16 / sizeof(T), PER = 256 * V;
+    const T* p = reinterpret_cast<const T*>(data) + base;
+    const long left = n - base;
+    if (left >= 4 * PER) {
+        Quad<T> q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int v = 0; v < V; v += 2) {
+                acc0 = norm_add<MAX>(acc0, load_f32(q[j].v + v));
+                acc1 = norm_add<MAX>(acc1, load_f32(q[j].v + v + 1));
+            }
+    } else {
+        for (long i = threadIdx.x; i < left; i += 256) acc0 = norm_add<MAX>(acc0, load_f32(p + i));
+    }
+}
+
 template <bool MAX>
 __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restrict__ partial)
 {
     __shared__ double lds[4];
-    double acc = 0.0;
+    double acc = 0.0, acc1 = 0.0;
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const GradSeg s = grad_seg(a, unit);
-        const long per = GN_UNIT / (s.dtype == VR_F32 ? 4 : 2);
-        const long base = (long)(unit - s.unit0) * per, end = base + per < s.n ? base + per : s.n;
-        for (long i = base + threadIdx.x; i < end; i += 256) acc = norm_add<MAX>(acc, grad_value(s.data, i, s.dtype));
+        const long at = (long)(unit - s.unit0) * GN_UNIT;
+        if (s.dtype == VR_F32) norm_unit<MAX, float>(s.data, at / 4, s.n, acc, acc1);
+        else if (s.dtype == VR_BF16) norm_unit<MAX, bf16>(s.data, at / 2, s.n, acc, acc1);
+        else norm_unit<MAX, __half>(s.data, at / 2, s.n, acc, acc1);
     }
-    acc = norm_block<MAX>(acc, lds);
+    acc = norm_block<MAX>(norm_join<MAX>(acc, acc1), lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
@@ -125,16 +140,89 @@ __global__ void __launch_bounds__(1024) k_grad_norm_finish(const double* __restr
     if (threadIdx.x == 0) norm[0] = norm_value<MAX>(acc);
 }
 
+template <typename T>
+__device__ __forceinline__ void scale_unit(void* data, long base, long n, float c)
+{
+    constexpr int V = 16 / sizeof(T), PER = 256 * V;
+    T* p = reinterpret_cast<T*>(data) + base;
+    const long left = n - base;
+    if (left >= 4 * PER) {
+        Quad<T> q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) store_f32(q[j].v + v, c * load_f32(q[j].v + v));
+            *reinterpret_cast<Quad<T>*>(p + j * PER + threadIdx.x * V) = q[j];
+        }
+    } else {
+        for (long i = threadIdx.x; i < left; i += 256) store_f32(p + i, c * load_f32(p + i));
+    }
+}
+
+// From the last unit to the first: the norm's pass ended there, and what it read last is still in the memory-side cache.
 __global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, const float* __restrict__ norm, float max_norm)
 {
     const float c = clip_factor(*norm, max_norm);
     if (c == 1.0f) return;
-    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+    for (int k = blockIdx.x; k < a.units; k += gridDim.x) {
+        const int unit = a.units - 1 - k;
         const GradSeg s = grad_seg(a, unit);
-        const long per = GN_UNIT / (s.dtype == VR_F32 ? 4 : 2);
-        const long base = (long)(unit - s.unit0) * per, end = base + per < s.n ? base + per : s.n;
-        for (long i = base + threadIdx.x; i < end; i += 256) grad_scale(s.data, i, s.dtype, c);
+        const long at = (long)(unit - s.unit0) * GN_UNIT;
+        if (s.dtype == VR_F32) scale_unit<float>(s.data, at / 4, s.n, c);
+        else if (s.dtype == VR_BF16) scale_unit<bf16>(s.data, at / 2, s.n, c);
+        else scale_unit<__half>(s.data, at / 2, s.n, c);
     }
+}
+
+// A handful of small tensors -- the pose corrections of a frame -- by one workgroup: a wave per tensor, the norm, and (CLIP)
+// the scaling, in one launch instead of three.
+constexpr int GN_SMALL = 2048;             // values of one tensor, at most: 32 a lane
+constexpr int GN_SMALL_ALL = 16384;        // of all of them
+template <bool MAX, bool CLIP>
+__global__ void __launch_bounds__(1024) k_grad_norm_small(GradArgs a, float max_norm, float* __restrict__ norm)
+{
+    __shared__ double lds[16];
+    __shared__ float factor;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    double acc = 0.0;
+    for (int t = w; t < a.count; t += 16) {
+        const GradSeg s = a.seg[t];
+        for (int i = lane; i < (int)s.n; i += 64)
+            acc = norm_add<MAX>(acc, s.dtype == VR_F32 ? load_f32(reinterpret_cast<const float*>(s.data) + i)
+                                     : s.dtype == VR_BF16 ? load_f32(reinterpret_cast<const bf16*>(s.data) + i)
+                                                          : load_f32(reinterpret_cast<const __half*>(s.data) + i));
+    }
+    acc = norm_block<MAX>(acc, lds);
+    if (threadIdx.x == 0) {
+        const float x = norm_value<MAX>(acc);
+        norm[0] = x;
+        factor = CLIP ? clip_factor(x, max_norm) : 1.0f;
+    }
+    if (!CLIP) return;
+    __syncthreads();
+    const float c = factor;
+    if (c == 1.0f) return;
+    for (int t = w; t < a.count; t += 16) {
+        const GradSeg s = a.seg[t];
+        for (int i = lane; i < (int)s.n; i += 64) {
+            if (s.dtype == VR_F32) { float* p = reinterpret_cast<float*>(s.data) + i; store_f32(p, c * load_f32(p)); }
+            else if (s.dtype == VR_BF16) { bf16* p = reinterpret_cast<bf16*>(s.data) + i; store_f32(p, c * load_f32(p)); }
+            else { __half* p = reinterpret_cast<__half*>(s.data) + i; store_f32(p, c * load_f32(p)); }
+        }
+    }
+}
+
+static bool small_grads(const VrGradTensor* t, int32_t count)
+{
+    int64_t all = 0, used = 0;
+    for (int i = 0; i < count; ++i) {
+        if (t[i].n > GN_SMALL) return false;
+        all += t[i].n;
+        used += t[i].n > 0;
+    }
+    return used <= GN_MAX_T && all <= GN_SMALL_ALL;
 }
 
 static int check_grads(const VrGradTensor* t, int32_t count)
@@ -166,11 +254,20 @@ static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
     return next;
 }
 
+// `clip`: scale as well, where one launch does both
 template <bool MAX>
 static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
-                     float* norm, double* partial, hipStream_t s)
+                     float* norm, double* partial, hipStream_t s, bool clip = false, float max_norm = 0.0f)
 {
     int n = 0;
+    if (n_factors == 0 && small_grads(tensors, count)) {
+        GradArgs a;
+        fill_grads(tensors, 0, count, a);
+        if (clip) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm_small<MAX, true>), dim3(1), dim3(1024), 0, s, a, max_norm, norm);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm_small<MAX, false>), dim3(1), dim3(1024), 0, s, a, max_norm, norm);
+        if (hipGetLastError() != hipSuccess) { set_error("grad norm: kernel launch failed"); return VR_ERR_HIP; }
+        return VR_OK;
+    }
     for (int first = 0; first < count;) {
         GradArgs a;
         first = fill_grads(tensors, first, count, a);
@@ -217,8 +314,8 @@ extern "C" int64_t vr_grad_norm_scratch_bytes(int32_t count, int32_t n_factors)
     return (launches > 0 ? launches : 1) * GN_GRID * (int64_t)sizeof(double);
 }
 
-extern "C" int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
-                            int32_t norm_type, float* norm, void* scratch, void* stream)
+static int check_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
+                      int32_t norm_type, const float* norm, const void* scratch)
 {
     if (int rc = check_grads(tensors, count)) return rc;
     if (n_factors < 0 || (n_factors > 0 && !factors) || !norm || !scratch || ((uintptr_t)scratch & 7) || (norm_type != 2 && norm_type != 0))
@@ -229,6 +326,13 @@ extern "C" int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const Vr
         if (int rc = sh_factor_args(a, f.means3D, f.P, f.campos, f.factors, f.n_views, f.factor_view_stride, f.sh_degree,
                                     (f.sh_degree + 1) * (f.sh_degree + 1), f.scale)) return rc;
     }
+    return VR_OK;
+}
+
+extern "C" int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
+                            int32_t norm_type, float* norm, void* scratch, void* stream)
+{
+    if (int rc = check_norm(tensors, count, factors, n_factors, norm_type, norm, scratch)) return rc;
     return norm_type == 2 ? grad_norm<false>(tensors, count, factors, n_factors, norm, (double*)scratch, (hipStream_t)stream)
                           : grad_norm<true>(tensors, count, factors, n_factors, norm, (double*)scratch, (hipStream_t)stream);
 }
@@ -244,6 +348,10 @@ extern "C" int vr_clip_grad_norm(const VrGradTensor* tensors, int32_t count, int
                                  void* scratch, void* stream)
 {
     if (!(max_norm >= 0.0f)) { set_error("clip: max_norm must not be negative or NaN"); return VR_ERR_INVALID_ARGUMENT; }
-    if (int rc = vr_grad_norm(tensors, count, nullptr, 0, norm_type, norm, scratch, stream)) return rc;
+    if (int rc = check_norm(tensors, count, nullptr, 0, norm_type, norm, scratch)) return rc;
+    const bool one = small_grads(tensors, count);
+    int rc = norm_type == 2 ? grad_norm<false>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, one, max_norm)
+                            : grad_norm<true>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, one, max_norm);
+    if (rc || one) return rc;
     return clip_grads(tensors, count, norm, max_norm, (hipStream_t)stream);
 }
