@@ -4,6 +4,7 @@ There is no fallback: if the HIP library is missing or does not export the ABI, 
 product path raises.  PyTorch is plumbing here (device memory, current stream); the signatures
 crossing the boundary are plain pointers and sizes.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -99,7 +100,7 @@ class VrShAdamTensor(C.Structure):
                 ("step", C.c_int64)]
 
 
-# VrGradTensor {data, n, dtype} is three 64-bit words: lists of them cross as flat int64 arrays
+# VrGradTensor {data, n, dtype} is three 64-bit words and VrAdamTensor eight: lists of them cross as packed bytes
 VR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # VrDataType
 
 
@@ -217,7 +218,7 @@ def load():
     lib.vr_training_loss_backward.argtypes = [vp, vp, i32, i32, i32, vp, vp, vp, vp, C.POINTER(C.c_float), C.c_float, C.c_float,
                                               i32, vp, vp, vp, vp, vp]
     lib.vr_adam_step.restype = C.c_int
-    lib.vr_adam_step.argtypes = [C.POINTER(VrAdamTensor), i32, C.c_double, C.c_double, C.c_double, vp]
+    lib.vr_adam_step.argtypes = [vp, i32, C.c_double, C.c_double, C.c_double, vp]
     lib.vr_densify_stats.restype = C.c_int
     lib.vr_densify_stats.argtypes = [vp, vp, i32, vp, vp, vp, vp]
     lib.vr_densify_plan_words.restype = C.c_int64
@@ -233,17 +234,16 @@ def load():
     lib.vr_sh_adam_step.restype = C.c_int
     lib.vr_sh_adam_step.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
                                     C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp]
-    i64p = C.POINTER(C.c_int64)
     lib.vr_grad_norm_scratch_bytes.restype = C.c_int64
     lib.vr_grad_norm_scratch_bytes.argtypes = [i32, i32]
     lib.vr_grad_norm.restype = C.c_int
-    lib.vr_grad_norm.argtypes = [i64p, i32, C.POINTER(VrShGradFactors), i32, i32, vp, vp, vp]
+    lib.vr_grad_norm.argtypes = [vp, i32, C.POINTER(VrShGradFactors), i32, i32, vp, vp, vp]
     lib.vr_clip_grads.restype = C.c_int
-    lib.vr_clip_grads.argtypes = [i64p, i32, vp, C.c_float, vp]
+    lib.vr_clip_grads.argtypes = [vp, i32, vp, C.c_float, vp]
     lib.vr_clip_grad_norm.restype = C.c_int
-    lib.vr_clip_grad_norm.argtypes = [i64p, i32, i32, C.c_float, vp, vp, vp]
+    lib.vr_clip_grad_norm.argtypes = [vp, i32, i32, C.c_float, vp, vp, vp]
     lib.vr_adam_step_clipped.restype = C.c_int
-    lib.vr_adam_step_clipped.argtypes = [C.POINTER(VrAdamTensor), i32, C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
+    lib.vr_adam_step_clipped.argtypes = [vp, i32, C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
     lib.vr_sh_adam_step_clipped.restype = C.c_int
     lib.vr_sh_adam_step_clipped.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
                                             C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
@@ -317,6 +317,19 @@ def ptr(t):
     if t is None or t.numel() == 0:
         return None
     return t.data_ptr()
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on(device):
+    """torch.cuda.device(device), which is a context of its own only where another device is current."""
+    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream_of(device):
+    """torch.cuda.current_stream(device).cuda_stream without the Stream object (2 us of a call that takes 10)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class Arena:

@@ -44,12 +44,12 @@ def _arguments(table, ids, scale, width, out_dtype):
 
 def _forward(table, ids, scale, width, dtype):
     device = table.device
-    with torch.cuda.device(device):
+    with _capi.on(device):
         out = torch.empty(ids.shape + table.shape[1:], dtype=dtype, device=device)
         if out.numel():
             lookup, keep = _arguments(table, ids, scale, width, dtype)
             _capi.check(_capi.load().vr_lookup_forward(C.byref(lookup), out.data_ptr(),
-                                                       torch.cuda.current_stream(device).cuda_stream))
+                                                       _capi.stream_of(device)))
     return out
 
 
@@ -71,7 +71,7 @@ class _Lookup(torch.autograd.Function):
         shape, dtype, device = ctx.like
         width = ctx.width
         want_table, want_scale = ctx.needs_input_grad[0], ctx.needs_input_grad[2]
-        with torch.cuda.device(device):
+        with _capi.on(device):
             d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
             d_scale = torch.empty(ids.shape, dtype=torch.float32, device=device) if want_scale else None
             if width == 0 or ids.numel() == 0:
@@ -86,7 +86,7 @@ class _Lookup(torch.autograd.Function):
                 nbytes = lib.vr_lookup_scratch_bytes(ids.numel(), shape[0], width)
                 scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
             _capi.check(lib.vr_lookup_backward(C.byref(lookup), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
-                                               _capi.ptr(scratch), nbytes, torch.cuda.current_stream(device).cuda_stream))
+                                               _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
         return d_table, None, d_scale, None, None
 
 

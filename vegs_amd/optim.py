@@ -19,6 +19,7 @@ GPU tensors only; there is no CPU path.
 """
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -43,50 +44,47 @@ class Adam(torch.optim.Optimizer):
         return loss
 
 
-def _validate(optimizer):
-    """Everything _collect would raise for, checked WITHOUT touching the optimizer: step_many validates every optimizer of
-    its batch before the first step counter moves, so an exception leaves all of them exactly as they were (a half-advanced
-    batch would skew the bias correction of a retry and desynchronise the ranks of a distributed job)."""
+def _entries(optimizer):
+    """[(parameter, gradient, group, its state or None)] of one optimizer (vegs_amd.optim.Adam or torch.optim.Adam: same
+    state layout), parameters without a gradient left out -- with everything checked WITHOUT touching the optimizer: step_many
+    goes through every optimizer of its batch before the first step counter moves, so an exception leaves all of them exactly
+    as they were (a half-advanced batch would skew the bias correction of a retry and desynchronise the ranks of a
+    distributed job)."""
+    out = []
     for group in optimizer.param_groups:
         if group.get("weight_decay", 0) != 0 or group.get("amsgrad", False) or group.get("maximize", False):
             raise NotImplementedError("the fused Adam covers the reference's configuration: no weight decay, no amsgrad")
         for p in group["params"]:
-            if p.grad is None:
+            g = p.grad
+            if g is None:
                 continue
             if not p.is_cuda:
                 raise ValueError("fused Adam expects GPU parameters (there is no CPU path)")
-            if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or p.grad.is_sparse:
+            if p.dtype != torch.float32 or g.dtype != torch.float32 or g.is_sparse:
                 raise ValueError("fused Adam expects dense float32 parameters and gradients")
             if not p.is_contiguous():
                 raise ValueError("fused Adam expects contiguous parameters")
-            st = optimizer.state.get(p) or {}
-            if len(st):
-                m, v = st.get("exp_avg"), st.get("exp_avg_sq")
-                if (m is None or v is None or "step" not in st or m.shape != p.shape or v.shape != p.shape
+            st = optimizer.state.get(p) or None
+            if st is not None:
+                m, v, shape = st.get("exp_avg"), st.get("exp_avg_sq"), p.shape
+                if (m is None or v is None or "step" not in st or m.shape != shape or v.shape != shape
                         or not m.is_contiguous() or not v.is_contiguous()):
                     raise ValueError("optimizer state does not match its parameter")
+            out.append((p, g, group, st))
+    return out
 
 
-def _collect(optimizer, by_cfg, keep):
-    """The VrAdamTensor entries of one VALIDATED optimizer (vegs_amd.optim.Adam or torch.optim.Adam: same state layout), its
-    step counters advanced as torch.optim.Adam.step does; parameters without a gradient are skipped."""
-    for group in optimizer.param_groups:
-        b1, b2 = group["betas"]
-        for p in group["params"]:
-            if p.grad is None:
-                continue
-            st = optimizer.state[p]
-            if len(st) == 0:
-                st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            m, v = st["exp_avg"], st["exp_avg_sq"]
-            st["step"] += 1
-            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
-            keep.append(g)
-            by_cfg.setdefault((p.device, float(b1), float(b2)), []).append(
-                _capi.VrAdamTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
-                                   float(group["lr"]), int(st["step"].item()), float(group["eps"])))
+def _advance(step):
+    """step += 1 on a state's counter, and its new value as a number."""
+    if step.is_cuda or step.dtype != torch.float32:
+        step += 1
+        return int(step.item())
+    n = step.numpy()                     # (the tensor's own memory: half the time of the addition through torch)
+    n += 1
+    return int(n)
+
+
+_ADAM = struct.Struct("4Qqdqd")           # VrAdamTensor
 
 
 def _grads_of(parameters):
@@ -94,13 +92,13 @@ def _grads_of(parameters):
     the scaling's workgroups on one gradient would race.)"""
     if isinstance(parameters, (torch.Tensor, torch.optim.Optimizer)):
         parameters = [parameters]
-    out = {}
+    grads = []
     for p in parameters:
-        for q in ([t for g in p.param_groups for t in g["params"]] if isinstance(p, torch.optim.Optimizer) else (p,)):
-            g = q.grad
-            if g is not None:
-                out[g.data_ptr(), g.numel()] = g
-    return list(out.values())
+        if isinstance(p, torch.Tensor):
+            grads.append(p.grad)
+        else:
+            grads += [q.grad for group in p.param_groups for q in group["params"]]
+    return list({(g.data_ptr(), g.numel()): g for g in grads if g is not None}.values())
 
 
 def _dense(t):
@@ -117,16 +115,17 @@ def _dense(t):
 
 
 def _grad_table(grads):
-    """(flat VrGradTensor words, device) of validated gradients that fill their memory."""
-    flat, device, dtypes = [], grads[0].device, _capi.VR_DTYPES
+    """(flat VrGradTensor words, device) of gradients that fill their memory, checked."""
+    device, kinds = grads[0].device, _capi.VR_DTYPES
+    if not grads[0].is_cuda or len({g.get_device() for g in grads}) != 1:
+        raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
+    flat = []
     for g in grads:
-        if g.device != device or not g.is_cuda:
-            raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
-        kind = dtypes.get(g.dtype)
-        if kind is None or g.layout != torch.strided:
+        kind = kinds.get(g.dtype)
+        if kind is None or g.layout is not torch.strided:
             raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.dtype}, {g.layout})")
         flat += (g.data_ptr(), g.numel(), kind)
-    return (C.c_int64 * len(flat))(*flat), device
+    return struct.pack("%dq" % len(flat), *flat), device
 
 
 def _norm_kind(norm_type):
@@ -172,11 +171,11 @@ def grad_norm(parameters, norm_type=2.0, sh_factors=()):
         return torch.tensor(0.0)
     table, device = _grad_table(keep) if keep else (None, items[0][1].device)
     lib = _capi.load()
-    with torch.cuda.device(device):
+    with _capi.on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
         scratch = _scratch(lib, len(keep), len(items), device)
         _capi.check(lib.vr_grad_norm(table, len(keep), (_capi.VrShGradFactors * len(items))(*[i[0] for i in items]), len(items),
-                                     kind, norm.data_ptr(), scratch.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+                                     kind, norm.data_ptr(), scratch.data_ptr(), _capi.stream_of(device)))
     return norm
 
 
@@ -203,10 +202,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             copies.append((g, grads[i]))
     table, device = _grad_table(grads)
     lib = _capi.load()
-    with torch.cuda.device(device):
+    with _capi.on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
         scratch = _scratch(lib, len(grads), 0, device)
-        stream = torch.cuda.current_stream(device).cuda_stream
+        stream = _capi.stream_of(device)
         if error_if_nonfinite:
             _capi.check(lib.vr_grad_norm(table, len(grads), None, 0, kind, norm.data_ptr(), scratch.data_ptr(), stream))
             if not math.isfinite(norm.item()):
@@ -245,30 +244,38 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
     else:
         max_grad_norm = _check_max_norm(max_grad_norm)
     lib = _capi.load()
-    for opt in optimizers:
-        _validate(opt)
+    batch = [(opt, _entries(opt)) for opt in optimizers]
     norm = None
     if max_grad_norm is not None:
-        devices = {p.device for opt in optimizers for g in opt.param_groups for p in g["params"] if p.grad is not None}
+        devices = {p.device for _, entries in batch for p, _, _, _ in entries}
         if len(devices) > 1:
             raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
-        if grad_norm is not None:
-            for device in devices:
-                _check_norm(grad_norm, device)
-            norm = grad_norm
-        else:
-            norm = _grad_norm(optimizers)
+        for device in devices if grad_norm is not None else ():
+            _check_norm(grad_norm, device)
+        norm = grad_norm if grad_norm is not None else _grad_norm(optimizers)
     by_cfg, keep = {}, []
-    for opt in optimizers:
-        _collect(opt, by_cfg, keep)
+    for opt, entries in batch:
+        for p, g, group, st in entries:
+            if st is None:
+                st = opt.state[p]
+                if len(st) == 0:
+                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            b1, b2 = group["betas"]
+            by_cfg.setdefault((p.device, float(b1), float(b2)), []).append(
+                _ADAM.pack(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), p.numel(),
+                           float(group["lr"]), _advance(st["step"]), float(group["eps"])))
     for (device, b1, b2), items in by_cfg.items():
-        arr = (_capi.VrAdamTensor * len(items))(*items)
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream(device).cuda_stream
+        with _capi.on(device):
             if norm is None:
-                rc = lib.vr_adam_step(arr, len(items), b1, b2, -1.0, stream)
+                rc = lib.vr_adam_step(b"".join(items), len(items), b1, b2, -1.0, _capi.stream_of(device))
             else:
-                rc = lib.vr_adam_step_clipped(arr, len(items), b1, b2, -1.0, norm.data_ptr(), max_grad_norm, stream)
+                rc = lib.vr_adam_step_clipped(b"".join(items), len(items), b1, b2, -1.0, norm.data_ptr(), max_grad_norm,
+                                              _capi.stream_of(device))
         _capi.check(rc)
     return norm
 
