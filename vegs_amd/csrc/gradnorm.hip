@@ -15,7 +15,8 @@
 namespace vr {
 
 constexpr int GN_MAX_T = 128;              // tensors per launch: the table is a kernel argument, 128 x 24 B of its 4 KB
-constexpr int GN_UNIT = 256 * 16 * 4;      // bytes a workgroup handles at a time: 256 threads x 16 B x 4
+constexpr int GN_LOADS = 4;                // 16-byte loads a thread has in flight, so a workgroup's unit is 16 KB; 4 KB units
+constexpr int GN_LOAD_BYTES = 256 * 16;    // (one load) where that would leave CUs without work
 constexpr int GN_GRID = 2048;              // workgroups of a launch at most: eight for each of the 256 CUs
 
 struct GradSeg {
@@ -26,40 +27,44 @@ struct GradSeg {
 };
 struct GradArgs {
     GradSeg seg[GN_MAX_T];
-    int count, units;
+    int count, units, loads;
 };
 
 // 16 bytes of values at an address of their own alignment (a gradient may be a view that starts anywhere)
 template <typename T>
 struct __attribute__((packed)) Quad { T v[16 / sizeof(T)]; };
 
-// the norm's accumulator: a sum of squares, or the largest magnitude (a NaN, once met, stays)
-template <bool MAX>
-__device__ __forceinline__ double norm_add(double acc, float x)
-{
-    if (MAX) { const float m = (float)acc, y = fabsf(x); return (y > m || y != y) ? (double)y : acc; }
-    return fma((double)x, (double)x, acc);
-}
-template <bool MAX>
-__device__ __forceinline__ double norm_join(double a, double b)
-{
-    if (MAX) return (b > a || b != b) ? b : a;
-    return a + b;
-}
-// over the workgroup's waves, in a fixed order; the result is thread 0's.  lds: one double per wave
-template <bool MAX>
-__device__ __forceinline__ double norm_block(double acc, double* lds)
+// the norm's accumulator: a sum of squares in fp64, or the largest magnitude in fp32 (a NaN, once met, stays)
+template <bool MAX> struct Acc { using type = double; };
+template <> struct Acc<true> { using type = float; };
+
+__device__ __forceinline__ double norm_add(double acc, float x) { return fma((double)x, (double)x, acc); }
+__device__ __forceinline__ double norm_join(double a, double b) { return a + b; }
+__device__ __forceinline__ float norm_join(float a, float b) { return (b > a || b != b) ? b : a; }
+__device__ __forceinline__ float norm_add(float acc, float x) { return norm_join(acc, fabsf(x)); }
+__device__ __forceinline__ float norm_value(double acc) { return (float)sqrt(acc); }
+__device__ __forceinline__ float norm_value(float acc) { return acc; }
+
+// over the workgroup's waves, in a fixed order; the result is thread 0's.  lds: one value per wave
+template <typename T>
+__device__ __forceinline__ T norm_block(T acc, T* lds)
 {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) acc = norm_join<MAX>(acc, __shfl_xor(acc, d, 64));
+    for (int d = 32; d > 0; d >>= 1) acc = norm_join(acc, __shfl_xor(acc, d, 64));
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = acc;
     __syncthreads();
     if (threadIdx.x == 0)
-        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) acc = norm_join<MAX>(acc, lds[w]);
+        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) acc = norm_join(acc, lds[w]);
     return acc;
 }
+// the workgroups' partial results, by one workgroup of 256 threads: always in this order
 template <bool MAX>
-__device__ __forceinline__ float norm_value(double acc) { return MAX ? (float)acc : (float)sqrt(acc); }
+__device__ __forceinline__ float norm_total(const double* __restrict__ partial, int n, typename Acc<MAX>::type* lds)
+{
+    typename Acc<MAX>::type acc = 0;
+    for (int i = threadIdx.x; i < n; i += 256) acc = norm_join(acc, (typename Acc<MAX>::type)partial[i]);
+    return norm_value(norm_block(acc, lds));
+}
 
 __device__ __forceinline__ GradSeg grad_seg(const GradArgs& a, int unit)
 {
@@ -71,43 +76,44 @@ __device__ __forceinline__ GradSeg grad_seg(const GradArgs& a, int unit)
     return a.seg[t];
 }
 
-// A unit's values: four loads of 16 bytes per thread at once where the unit is full, single values in a tensor's last unit.
+// A unit's values: LOADS loads of 16 bytes per thread at once where the unit is full, single values in a tensor's last unit.
 // Two accumulators, for the 64-bit multiply-add's latency.
-template <bool MAX, typename T>
-__device__ __forceinline__ void norm_unit(const void* data, long base, long n, double& acc0, double& acc1)
+template <typename T, int LOADS, typename A>
+__device__ __forceinline__ void norm_unit(const void* data, long base, long n, A& acc0, A& acc1)
 {
     constexpr int V = 16 / sizeof(T), PER = 256 * V;
     const T* p = reinterpret_cast<const T*>(data) + base;
     const long left = n - base;
-    if (left >= 4 * PER) {
-        Quad<T> q[4];
+    if (left >= LOADS * PER) {
+        Quad<T> q[LOADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+        for (int j = 0; j < LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < LOADS; ++j)
 #pragma unroll
             for (int v = 0; v < V; v += 2) {
-                acc0 = norm_add<MAX>(acc0, load_f32(q[j].v + v));
-                acc1 = norm_add<MAX>(acc1, load_f32(q[j].v + v + 1));
+                acc0 = norm_add(acc0, load_f32(q[j].v + v));
+                acc1 = norm_add(acc1, load_f32(q[j].v + v + 1));
             }
     } else {
-        for (long i = threadIdx.x; i < left; i += 256) acc0 = norm_add<MAX>(acc0, load_f32(p + i));
+        for (long i = threadIdx.x; i < left; i += 256) acc0 = norm_add(acc0, load_f32(p + i));      // (less than a unit)
     }
 }
 
-template <bool MAX>
+template <bool MAX, int LOADS>
 __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restrict__ partial)
 {
-    __shared__ double lds[4];
-    double acc = 0.0, acc1 = 0.0;
+    using A = typename Acc<MAX>::type;
+    __shared__ A lds[4];
+    A acc = 0, acc1 = 0;
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const GradSeg s = grad_seg(a, unit);
-        const long at = (long)(unit - s.unit0) * GN_UNIT;
-        if (s.dtype == VR_F32) norm_unit<MAX, float>(s.data, at / 4, s.n, acc, acc1);
-        else if (s.dtype == VR_BF16) norm_unit<MAX, bf16>(s.data, at / 2, s.n, acc, acc1);
-        else norm_unit<MAX, __half>(s.data, at / 2, s.n, acc, acc1);
+        const long at = (long)(unit - s.unit0) * (LOADS * GN_LOAD_BYTES);
+        if (s.dtype == VR_F32) norm_unit<float, LOADS>(s.data, at / 4, s.n, acc, acc1);
+        else if (s.dtype == VR_BF16) norm_unit<bf16, LOADS>(s.data, at / 2, s.n, acc, acc1);
+        else norm_unit<__half, LOADS>(s.data, at / 2, s.n, acc, acc1);
     }
-    acc = norm_block<MAX>(norm_join<MAX>(acc, acc1), lds);
+    acc = norm_block(norm_join(acc, acc1), lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
@@ -116,42 +122,41 @@ __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restric
 template <bool MAX>
 __global__ void __launch_bounds__(256) k_sh_grad_norm(ShFactorArgs a, double* __restrict__ partial)
 {
-    __shared__ double lds[4];
-    double acc = 0.0;
+    using A = typename Acc<MAX>::type;
+    __shared__ A lds[4];
+    A acc = 0;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < a.P; i += gridDim.x * 256) {
         float g[SHF_ROW_MAX];
 #pragma unroll
         for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = 0.0f;
         sh_row_from_factors(a, i, g);
 #pragma unroll
-        for (int q = 0; q < SHF_ROW_MAX; ++q) acc = norm_add<MAX>(acc, a.scale * g[q]);
+        for (int q = 0; q < SHF_ROW_MAX; ++q) acc = norm_add(acc, a.scale * g[q]);
     }
-    acc = norm_block<MAX>(acc, lds);
+    acc = norm_block(acc, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(1024) k_grad_norm_finish(const double* __restrict__ partial, int n, float* __restrict__ norm)
+__global__ void __launch_bounds__(256) k_grad_norm_finish(const double* __restrict__ partial, int n, float* __restrict__ norm)
 {
-    __shared__ double lds[16];
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) acc = norm_join<MAX>(acc, partial[i]);
-    acc = norm_block<MAX>(acc, lds);
-    if (threadIdx.x == 0) norm[0] = norm_value<MAX>(acc);
+    __shared__ typename Acc<MAX>::type lds[4];
+    const float x = norm_total<MAX>(partial, n, lds);
+    if (threadIdx.x == 0) norm[0] = x;
 }
 
-template <typename T>
+template <typename T, int LOADS>
 __device__ __forceinline__ void scale_unit(void* data, long base, long n, float c)
 {
     constexpr int V = 16 / sizeof(T), PER = 256 * V;
     T* p = reinterpret_cast<T*>(data) + base;
     const long left = n - base;
-    if (left >= 4 * PER) {
-        Quad<T> q[4];
+    if (left >= LOADS * PER) {
+        Quad<T> q[LOADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+        for (int j = 0; j < LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < LOADS; ++j) {
 #pragma unroll
             for (int v = 0; v < V; ++v) store_f32(q[j].v + v, c * load_f32(q[j].v + v));
             *reinterpret_cast<Quad<T>*>(p + j * PER + threadIdx.x * V) = q[j];
@@ -162,17 +167,34 @@ __device__ __forceinline__ void scale_unit(void* data, long base, long n, float 
 }
 
 // From the last unit to the first: the norm's pass ended there, and what it read last is still in the memory-side cache.
-__global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, const float* __restrict__ norm, float max_norm)
+// The norm comes from memory, or (KIND 1: sum of squares, 2: largest magnitude) from k_grad_norm's partial results, which every workgroup
+// adds up for itself -- at most 16 KB from the L2 each, and a launch less between the two passes.
+template <int KIND, int LOADS>
+__global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, float* __restrict__ norm, float max_norm,
+                                                    const double* __restrict__ partial, int n_partial)
 {
-    const float c = clip_factor(*norm, max_norm);
+    float c;
+    if (KIND) {
+        __shared__ typename Acc<KIND == 2>::type lds[4];
+        __shared__ float total;
+        const float x = norm_total<KIND == 2>(partial, n_partial, lds);
+        if (threadIdx.x == 0) {
+            total = x;
+            if (blockIdx.x == 0) norm[0] = x;
+        }
+        __syncthreads();
+        c = clip_factor(total, max_norm);
+    } else {
+        c = clip_factor(*norm, max_norm);
+    }
     if (c == 1.0f) return;
     for (int k = blockIdx.x; k < a.units; k += gridDim.x) {
         const int unit = a.units - 1 - k;
         const GradSeg s = grad_seg(a, unit);
-        const long at = (long)(unit - s.unit0) * GN_UNIT;
-        if (s.dtype == VR_F32) scale_unit<float>(s.data, at / 4, s.n, c);
-        else if (s.dtype == VR_BF16) scale_unit<bf16>(s.data, at / 2, s.n, c);
-        else scale_unit<__half>(s.data, at / 2, s.n, c);
+        const long at = (long)(unit - s.unit0) * (LOADS * GN_LOAD_BYTES);
+        if (s.dtype == VR_F32) scale_unit<float, LOADS>(s.data, at / 4, s.n, c);
+        else if (s.dtype == VR_BF16) scale_unit<bf16, LOADS>(s.data, at / 2, s.n, c);
+        else scale_unit<__half, LOADS>(s.data, at / 2, s.n, c);
     }
 }
 
@@ -183,20 +205,21 @@ constexpr int GN_SMALL_ALL = 16384;        // of all of them
 template <bool MAX, bool CLIP>
 __global__ void __launch_bounds__(1024) k_grad_norm_small(GradArgs a, float max_norm, float* __restrict__ norm)
 {
-    __shared__ double lds[16];
+    using A = typename Acc<MAX>::type;
+    __shared__ A lds[16];
     __shared__ float factor;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    double acc = 0.0;
+    A acc = 0;
     for (int t = w; t < a.count; t += 16) {
         const GradSeg s = a.seg[t];
         for (int i = lane; i < (int)s.n; i += 64)
-            acc = norm_add<MAX>(acc, s.dtype == VR_F32 ? load_f32(reinterpret_cast<const float*>(s.data) + i)
+            acc = norm_add(acc, s.dtype == VR_F32 ? load_f32(reinterpret_cast<const float*>(s.data) + i)
                                      : s.dtype == VR_BF16 ? load_f32(reinterpret_cast<const bf16*>(s.data) + i)
                                                           : load_f32(reinterpret_cast<const __half*>(s.data) + i));
     }
-    acc = norm_block<MAX>(acc, lds);
+    acc = norm_block(acc, lds);
     if (threadIdx.x == 0) {
-        const float x = norm_value<MAX>(acc);
+        const float x = norm_value(acc);
         norm[0] = x;
         factor = CLIP ? clip_factor(x, max_norm) : 1.0f;
     }
@@ -243,9 +266,14 @@ static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
 {
     int next = first;
     a.count = a.units = 0;
+    // one load a thread unless that fills the largest grid
+    int64_t bytes = 0;
+    for (int i = first; i < count && i < first + GN_MAX_T; ++i) bytes += t[i].n * (t[i].dtype == VR_F32 ? 4 : 2);
+    a.loads = bytes > (int64_t)GN_GRID * GN_LOAD_BYTES ? GN_LOADS : 1;
+    const long unit = (long)a.loads * GN_LOAD_BYTES;
     for (; next < count && a.count < GN_MAX_T; ++next) {
         if (t[next].n == 0) continue;
-        const long units = (t[next].n * (t[next].dtype == VR_F32 ? 4 : 2) + GN_UNIT - 1) / GN_UNIT;
+        const long units = (t[next].n * (t[next].dtype == VR_F32 ? 4 : 2) + unit - 1) / unit;
         if (a.units + units > 0x3fffffff) break;
         a.seg[a.count++] = GradSeg{t[next].data, (long)t[next].n, a.units, (int)t[next].dtype};
         a.units += (int)units;
@@ -254,7 +282,15 @@ static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
     return next;
 }
 
-// `clip`: scale as well, where one launch does both
+template <int KIND>
+static void launch_clip(const GradArgs& a, float* norm, float max_norm, const double* partial, int n, hipStream_t s)
+{
+    const dim3 grid(a.units < GN_GRID ? a.units : GN_GRID);
+    if (a.loads == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_clip_grads<KIND, 1>), grid, dim3(256), 0, s, a, norm, max_norm, partial, n);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_clip_grads<KIND, GN_LOADS>), grid, dim3(256), 0, s, a, norm, max_norm, partial, n);
+}
+
+// clip: scale as well
 template <bool MAX>
 static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFactors* factors, int32_t n_factors,
                      float* norm, double* partial, hipStream_t s, bool clip = false, float max_norm = 0.0f)
@@ -273,7 +309,8 @@ static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradF
         first = fill_grads(tensors, first, count, a);
         if (a.units == 0) continue;
         const int grid = a.units < GN_GRID ? a.units : GN_GRID;
-        hipLaunchKernelGGL(k_grad_norm<MAX>, dim3(grid), dim3(256), 0, s, a, partial + n);
+        if (a.loads == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm<MAX, 1>), dim3(grid), dim3(256), 0, s, a, partial + n);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm<MAX, GN_LOADS>), dim3(grid), dim3(256), 0, s, a, partial + n);
         n += grid;
     }
     for (int i = 0; i < n_factors; ++i) {
@@ -286,7 +323,15 @@ static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradF
         hipLaunchKernelGGL(k_sh_grad_norm<MAX>, dim3(grid), dim3(256), 0, s, a, partial + n);
         n += grid;
     }
-    hipLaunchKernelGGL(k_grad_norm_finish<MAX>, dim3(1), dim3(1024), 0, s, (const double*)partial, n, norm);
+    if (clip && n > 0) {
+        for (int first = 0; first < count;) {
+            GradArgs a;
+            first = fill_grads(tensors, first, count, a);
+            if (a.units > 0) launch_clip<MAX ? 2 : 1>(a, norm, max_norm, partial, n, s);
+        }
+    } else {
+        hipLaunchKernelGGL(k_grad_norm_finish<MAX>, dim3(1), dim3(256), 0, s, (const double*)partial, n, norm);
+    }
     if (hipGetLastError() != hipSuccess) { set_error("grad norm: kernel launch failed"); return VR_ERR_HIP; }
     return VR_OK;
 }
@@ -296,8 +341,7 @@ static int clip_grads(const VrGradTensor* tensors, int32_t count, const float* n
     for (int first = 0; first < count;) {
         GradArgs a;
         first = fill_grads(tensors, first, count, a);
-        if (a.units == 0) continue;
-        hipLaunchKernelGGL(k_clip_grads, dim3(a.units < GN_GRID ? a.units : GN_GRID), dim3(256), 0, s, a, norm, max_norm);
+        if (a.units > 0) launch_clip<0>(a, const_cast<float*>(norm), max_norm, nullptr, 0, s);
     }
     if (hipGetLastError() != hipSuccess) { set_error("clip: kernel launch failed"); return VR_ERR_HIP; }
     return VR_OK;
@@ -349,9 +393,6 @@ extern "C" int vr_clip_grad_norm(const VrGradTensor* tensors, int32_t count, int
 {
     if (!(max_norm >= 0.0f)) { set_error("clip: max_norm must not be negative or NaN"); return VR_ERR_INVALID_ARGUMENT; }
     if (int rc = check_norm(tensors, count, nullptr, 0, norm_type, norm, scratch)) return rc;
-    const bool one = small_grads(tensors, count);
-    int rc = norm_type == 2 ? grad_norm<false>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, one, max_norm)
-                            : grad_norm<true>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, one, max_norm);
-    if (rc || one) return rc;
-    return clip_grads(tensors, count, norm, max_norm, (hipStream_t)stream);
+    return norm_type == 2 ? grad_norm<false>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, true, max_norm)
+                          : grad_norm<true>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, true, max_norm);
 }
