@@ -31,11 +31,11 @@ typedef struct VrLookup {
 /* out [n, width], rows one after the other. */
 int vr_lookup_forward(const VrLookup* lookup, void* out, void* stream);
 
-/* Bytes of device scratch that vr_lookup_backward needs, for its sort by row (0: bad sizes). */
+/* Bytes of device scratch that vr_lookup_backward needs for the table's gradient (0: none -- few entries -- or bad sizes). */
 int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width);
 
 /* grad [n, width], rows grad_stride elements apart.  d_table [rows, width] in the table's type, every element written; NULL:
- * not wanted (scratch may be NULL then).  d_row_scale [n] fp32; NULL: not wanted.  Sums are fp32 (in pieces of a fixed size that are
+ * not wanted (scratch may be NULL then, and where no scratch is needed).  d_row_scale [n] fp32; NULL: not wanted.  Sums are fp32 (in pieces of a fixed size that are
  * joined in order: the same inputs give the same bits) and rounded once. */
 int vr_lookup_backward(const VrLookup* lookup, const void* grad, int64_t grad_stride, void* d_table, float* d_row_scale,
                        void* scratch, int64_t scratch_bytes, void* stream);

@@ -128,21 +128,22 @@ k_lookup_keys(LookupArgs a, uint32_t* __restrict__ key, uint32_t* __restrict__ v
     zero_fill(zero, zero_bytes, (long)(blockIdx.x - key_blocks) * 256 + threadIdx.x, (long)(gridDim.x - key_blocks) * 256);
 }
 
-// The same for up to SORT_SMALL entries, sorted as well: one workgroup holds them in LDS through all passes (stable, 8 bits each),
-// the others clear the gradient meanwhile.  One launch where the general sort takes a launch for the keys and four a pass: at
-// 16384 entries and 32000 rows 49 us of kernels, and as much again between them.
+constexpr uint32_t NO_ENTRY = 0xffffffffu;            // behind every row and behind "no row"
+
+// ---- the sort of few entries by one workgroup: all of them stay in LDS through the passes (stable, 8 bits each).
 constexpr int SORT_SMALL = 16384, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 
 template <int ITEMS>
-__global__ void __launch_bounds__(SORT_THREADS)
-k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict__ val_out, int bits, char* __restrict__ zero, long zero_bytes)
+struct SortLds {
+    uint32_t cnt[SORT_WAVES][256], base[256], wave_sum[4];
+    uint32_t key[SORT_THREADS * ITEMS], val[SORT_THREADS * ITEMS];
+};
+
+// Entries 0 .. n - 1 by their row (`rows` for "no row", padding behind it) into lds.key / lds.val.  All SORT_THREADS threads; the
+// arrays may be read when it returns.
+template <int ITEMS>
+__device__ __forceinline__ void sort_entries(const LookupArgs& a, int bits, SortLds<ITEMS>& lds)
 {
-    __shared__ uint32_t cnt[SORT_WAVES][256], base[256], wave_sum[4];
-    __shared__ uint32_t skey[SORT_THREADS * ITEMS], sval[SORT_THREADS * ITEMS];
-    if (blockIdx.x > 0) {
-        zero_fill(zero, zero_bytes, (long)(blockIdx.x - 1) * SORT_THREADS + threadIdx.x, (long)(gridDim.x - 1) * SORT_THREADS);
-        return;
-    }
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * ITEMS) + lane;
     const unsigned long long before = (1ull << lane) - 1ull;
     uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
@@ -150,11 +151,11 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
     for (int x = 0; x < ITEMS; ++x) {
         const int i = first + 64 * x;
         const long row = i < a.n ? row_of(a, i) : -1;
-        key[x] = i < a.n ? (row >= 0 ? (uint32_t)row : (uint32_t)a.rows) : 0xffffffffu;   // what is padding stays last
+        key[x] = i < a.n ? (row >= 0 ? (uint32_t)row : (uint32_t)a.rows) : NO_ENTRY;
         val[x] = (uint32_t)i;
     }
     for (int shift = 0; shift < bits; shift += 8) {
-        for (int d = threadIdx.x; d < SORT_WAVES * 256; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
+        for (int d = threadIdx.x; d < SORT_WAVES * 256; d += SORT_THREADS) (&lds.cnt[0][0])[d] = 0;
         __syncthreads();
         // the entry's place among those of its digit in its wave: lanes of the same digit by ballots, earlier items from the count
 #pragma unroll
@@ -166,10 +167,10 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
                 const unsigned long long on = __ballot((d >> b) & 1u);
                 same &= ((d >> b) & 1u) ? on : ~on;
             }
-            const uint32_t prior = cnt[w][d];
+            const uint32_t prior = lds.cnt[w][d];
             rank[x] = prior + (uint32_t)__popcll(same & before);
             __builtin_amdgcn_wave_barrier();
-            if ((same & before) == 0) cnt[w][d] = prior + (uint32_t)__popcll(same);
+            if ((same & before) == 0) lds.cnt[w][d] = prior + (uint32_t)__popcll(same);
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
@@ -177,8 +178,8 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
         uint32_t total = 0, incl = 0;
         if (threadIdx.x < 256) {
             for (int k = 0; k < SORT_WAVES; ++k) {
-                const uint32_t c = cnt[k][threadIdx.x];
-                cnt[k][threadIdx.x] = total;
+                const uint32_t c = lds.cnt[k][threadIdx.x];
+                lds.cnt[k][threadIdx.x] = total;
                 total += c;
             }
             incl = total;
@@ -187,32 +188,45 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
                 const uint32_t o = (uint32_t)__shfl_up((int)incl, dd, 64);
                 if (lane >= dd) incl += o;
             }
-            if (lane == 63) wave_sum[w] = incl;
+            if (lane == 63) lds.wave_sum[w] = incl;
         }
         __syncthreads();
         if (threadIdx.x < 256) {
             uint32_t b = incl - total;
-            for (int k = 0; k < w; ++k) b += wave_sum[k];
-            base[threadIdx.x] = b;
+            for (int k = 0; k < w; ++k) b += lds.wave_sum[k];
+            lds.base[threadIdx.x] = b;
         }
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < ITEMS; ++x) {
-            const uint32_t d = (key[x] >> shift) & 255u, at = base[d] + cnt[w][d] + rank[x];
-            skey[at] = key[x];
-            sval[at] = val[x];
+            const uint32_t d = (key[x] >> shift) & 255u, at = lds.base[d] + lds.cnt[w][d] + rank[x];
+            lds.key[at] = key[x];
+            lds.val[at] = val[x];
         }
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < ITEMS; ++x) {
-            key[x] = skey[first + 64 * x];
-            val[x] = sval[first + 64 * x];
+            key[x] = lds.key[first + 64 * x];
+            val[x] = lds.val[first + 64 * x];
         }
     }
-#pragma unroll
-    for (int x = 0; x < ITEMS; ++x) {
-        const int i = first + 64 * x;
-        if (i < a.n) { key_out[i] = key[x]; val_out[i] = val[x]; }
+}
+
+// First launch for up to SORT_SMALL entries: one workgroup sorts, the others clear the gradient meanwhile.  (The general sort takes a
+// launch for the keys and four a pass: at 16384 entries and 32000 rows 49 us of kernels, and as much again between them; this one 35.)
+template <int ITEMS>
+__global__ void __launch_bounds__(SORT_THREADS)
+k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict__ val_out, int bits, char* __restrict__ zero, long zero_bytes)
+{
+    __shared__ SortLds<ITEMS> lds;
+    if (blockIdx.x > 0) {
+        zero_fill(zero, zero_bytes, (long)(blockIdx.x - 1) * SORT_THREADS + threadIdx.x, (long)(gridDim.x - 1) * SORT_THREADS);
+        return;
+    }
+    sort_entries<ITEMS>(a, bits, lds);
+    for (int i = threadIdx.x; i < a.n; i += SORT_THREADS) {
+        key_out[i] = lds.key[i];
+        val_out[i] = lds.val[i];
     }
 }
 
@@ -227,7 +241,6 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
 //
 // The gradient rows are gathered: each is one contiguous read of width x 4 bytes, UNROLL of them in flight per lane.
 constexpr int UNROLL = 8;
-constexpr uint32_t NO_ENTRY = 0xffffffffu;
 
 struct SumArgs {
     const uint32_t *key, *val;
@@ -423,6 +436,123 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
     }
 }
 
+// ---- up to SMALL entries in one launch without any scratch: every workgroup sorts all of them in its LDS and writes the rows of its own
+// range, the ones without entries as zeros.  A row is one group's; one of more than SMALL_LONG entries is the whole workgroup's, in
+// contiguous pieces that are added in order.  (100 entries, 1000 rows of ten floats: 6 us against 12 for the three launches.)
+constexpr int SMALL = SORT_THREADS, SMALL_LONG = 32;
+
+__device__ __forceinline__ int first_at_least(const uint32_t* key, int n, uint32_t k)
+{
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (key[mid] < k) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+// acc += the entries j .. end - 1, all of the row at `table`
+template <typename TT, typename TO, int V, bool DSCALE>
+__device__ __forceinline__ void add_entries(const LookupArgs& a, const SumArgs& q, const uint32_t* val, int j, int end, long col, long want,
+                                            bool live, const TT* table, float (&acc)[V])
+{
+    const TO* grad = reinterpret_cast<const TO*>(q.grad) + col;
+    const int G = 1 << q.g_shift, lane = threadIdx.x & (G - 1);
+    Pack<TT, V> t;
+    if (DSCALE) t = *reinterpret_cast<const Pack<TT, V>*>(table);
+    for (; j < end; j += UNROLL) {
+        Pack<TO, V> g[UNROLL];
+        float s[UNROLL];
+#pragma unroll
+        for (int x = 0; x < UNROLL; ++x) {
+            const long i = val[j + x < end ? j + x : j];
+            s[x] = a.row_scale ? a.row_scale[i] : 1.0f;
+            g[x] = load_once<TO, V>(grad + i * q.grad_stride);
+        }
+#pragma unroll
+        for (int x = 0; x < UNROLL; ++x) {
+            if (j + x >= end) break;
+            const float sx = a.scale * s[x];
+            float dot = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float gv = load_f32(g[x].v + v);
+                acc[v] = fmaf(sx, gv, acc[v]);
+                if (DSCALE && live && col + v >= want) dot = fmaf(gv, load_f32(t.v + v), dot);
+            }
+            if (DSCALE) {
+                for (int w = G >> 1; w > 0; w >>= 1) dot += __shfl_xor(dot, w, 64);
+                if (lane == 0) q.d_row_scale[val[j + x]] = a.scale * dot;
+            }
+        }
+    }
+}
+
+template <typename TT, typename TO, int V, bool DSCALE>
+__global__ void __launch_bounds__(SORT_THREADS) k_lookup_small(LookupArgs a, SumArgs q, int bits, long rows_each)
+{
+    __shared__ SortLds<1> lds;
+    __shared__ float part[SORT_THREADS * V];
+    __shared__ int long_runs[SMALL / SMALL_LONG], n_long;
+    if (threadIdx.x == 0) n_long = 0;
+    sort_entries<1>(a, bits, lds);
+    const int n = (int)a.n, G = 1 << q.g_shift, lane = threadIdx.x & (G - 1), group = threadIdx.x >> q.g_shift, groups = SORT_THREADS >> q.g_shift;
+    const long r0 = (long)blockIdx.x * rows_each, r1 = r0 + rows_each < a.rows ? r0 + rows_each : a.rows;
+    const long want = ((long)blockIdx.y * G + lane) * V;
+    const bool live = want < a.width;
+    const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
+    const TT* table = reinterpret_cast<const TT*>(a.table) + col;
+    TT* d_table = reinterpret_cast<TT*>(q.d_table) + col;
+    const int e0 = first_at_least(lds.key, n, (uint32_t)r0), e1 = first_at_least(lds.key, n, (uint32_t)r1);
+    float acc[V];
+    // rows without entries
+    for (long r = r0 + group; r < r1; r += groups) {
+        const int at = first_at_least(lds.key, n, (uint32_t)r);
+        if (live && (at >= n || lds.key[at] != (uint32_t)r)) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+            store_row<TT, V>(d_table + r * a.width, acc);
+        }
+    }
+    if (DSCALE && blockIdx.x == 0)                               // entries without a row
+        for (int j = threadIdx.x; j < n; j += SORT_THREADS)
+            if (lds.key[j] >= (uint32_t)a.rows) q.d_row_scale[lds.val[j]] = 0.0f;
+    // rows with entries: the group of the row's first one
+    for (int j = e0 + group; j < e1; j += groups) {
+        const uint32_t k = lds.key[j];
+        if (j > e0 && lds.key[j - 1] == k) continue;
+        const int end = first_at_least(lds.key, n, k + 1);
+        if (end - j > SMALL_LONG) {
+            if (lane == 0) long_runs[atomicAdd(&n_long, 1)] = j;       // (their order does not matter: each is a row of its own)
+            continue;
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        add_entries<TT, TO, V, DSCALE>(a, q, lds.val, j, end, col, want, live, table + (long)k * a.table_stride, acc);
+        if (live) store_row<TT, V>(d_table + (long)k * a.width, acc);
+    }
+    __syncthreads();
+    for (int o = 0; o < n_long; ++o) {
+        const int j = long_runs[o];
+        const uint32_t k = lds.key[j];
+        const int end = first_at_least(lds.key, n, k + 1), each = (end - j + groups - 1) / groups;
+        const int from = j + group * each, upto = from + each < end ? from + each : end;
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+        if (from < upto) add_entries<TT, TO, V, DSCALE>(a, q, lds.val, from, upto, col, want, live, table + (long)k * a.table_stride, acc);
+#pragma unroll
+        for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
+        __syncthreads();
+        if (group == 0 && live) {
+            for (int g = 1; g < groups && g * each < end - j; ++g)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[v] += part[((g << q.g_shift) + lane) * V + v];
+            store_row<TT, V>(d_table + (long)k * a.width, acc);
+        }
+        __syncthreads();
+    }
+}
+
 // The scales' gradient alone, entry by entry: where the table's is not wanted, or the width takes more than one tile.
 template <typename TT, typename TO, int V>
 __global__ void __launch_bounds__(256) k_lookup_dscale(LookupArgs a, const TO* __restrict__ grad, long grad_stride,
@@ -527,7 +657,13 @@ struct Backward {
     static void launch(const LookupArgs& a, const SumArgs& q, const Tiling& t, hipStream_t s)
     {
         const bool fused = q.d_row_scale && q.d_table && t.tiles == 1;
-        if (q.d_table) {
+        if (q.d_table && a.n <= SMALL) {
+            // (a row's columns may take several workgroups: 256 ranges of rows, or fewer)
+            const long rows_each = (a.rows + 255) / 256;
+            const dim3 grid((unsigned)((a.rows + rows_each - 1) / rows_each), t.tiles);
+            if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_small<TT, TO, V, true>), grid, dim3(SORT_THREADS), 0, s, a, q, key_bits(a.rows), rows_each);
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_small<TT, TO, V, false>), grid, dim3(SORT_THREADS), 0, s, a, q, key_bits(a.rows), rows_each);
+        } else if (q.d_table) {
             const dim3 grid((unsigned)(((t.chunks << t.g_shift) + 255) / 256), t.tiles);
             if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, true>), grid, dim3(256), 0, s, a, q);
             else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, false>), grid, dim3(256), 0, s, a, q);
@@ -578,7 +714,7 @@ static size_t slots_bytes(int64_t n, int64_t width)
 extern "C" int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width)
 {
     if (n < 0 || n >= (1ll << 30) || rows < 0 || rows >= 0x7fffffffll || width < 1 || width > (1 << 24)) return 0;
-    if (n == 0) n = 1;
+    if (n <= SMALL) return 0;
     return (int64_t)(4 * align_up((size_t)n * 4, 256) + align_up(sort_pairs_scratch_bytes((long)n), 256) + slots_bytes(n, width));
 }
 
@@ -591,22 +727,21 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
     if ((a.n > 0 && !grad) || ((uintptr_t)grad & (element - 1)) || grad_stride < a.width || grad_stride > (1ll << 40) ||
         ((uintptr_t)d_table & (t_element - 1)) || ((uintptr_t)d_row_scale & 3))
         { set_error("lookup: grad is required, arrays aligned to their elements, grad_stride >= width"); return VR_ERR_INVALID_ARGUMENT; }
-    if (d_table && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < vr_lookup_scratch_bytes(a.n, a.rows, a.width)))
+    if (d_table && a.n > SMALL && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < vr_lookup_scratch_bytes(a.n, a.rows, a.width)))
         { set_error("lookup: the table's gradient needs vr_lookup_scratch_bytes of scratch, 256-byte aligned"); return VR_ERR_INVALID_ARGUMENT; }
     if (a.rows == 0) d_table = nullptr;
     if (!d_table && (!d_row_scale || a.n == 0)) return VR_OK;
     hipStream_t s = (hipStream_t)stream;
     SumArgs q{nullptr, nullptr, grad, (long)grad_stride, d_table, d_row_scale, nullptr, 0, 0};
-    if (d_table) {
-        const size_t arr = align_up((size_t)(a.n > 0 ? a.n : 1) * 4, 256);
+    if (d_table && a.n > SMALL) {
+        const size_t arr = align_up((size_t)a.n * 4, 256);
         char* base = (char*)scratch;
         uint32_t *k0 = (uint32_t*)base, *v0 = (uint32_t*)(base + arr), *k1 = (uint32_t*)(base + 2 * arr), *v1 = (uint32_t*)(base + 3 * arr);
         const long zero_bytes = a.rows * a.width * (long)t_element, zero_blocks = (zero_bytes + 16383) / 16384;
-        if (a.n > 0 && a.n <= SORT_SMALL) {
+        if (a.n <= SORT_SMALL) {
             const dim3 grid(1 + (unsigned)(zero_blocks < 1024 ? zero_blocks : 1024));
             const int bits = key_bits(a.rows);
-            if (a.n <= SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<1>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
-            else if (a.n <= 4 * SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
+            if (a.n <= 4 * SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
             else hipLaunchKernelGGL(k_lookup_sort<16>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
             VR_KERNEL_CHECK("lookup_sort", s, false);
             q.key = k0;
@@ -616,7 +751,6 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
             hipLaunchKernelGGL(k_lookup_keys, dim3(key_blocks + (unsigned)(zero_blocks < 4096 ? zero_blocks : 4096)), dim3(256), 0, s, a, k0,
                                v0, key_blocks, (char*)d_table, zero_bytes);
             VR_KERNEL_CHECK("lookup_keys", s, false);
-            if (a.n == 0) return VR_OK;
             int where = 0;
             if (int rc = launch_sort_pairs(k0, v0, k1, v1, a.n, 0u, key_bits(a.rows), base + 4 * arr, s, false, &where)) return rc;
             q.key = where ? k1 : k0;

@@ -84,7 +84,7 @@ class _Lookup(torch.autograd.Function):
             scratch, nbytes = None, 0
             if want_table:
                 nbytes = lib.vr_lookup_scratch_bytes(ids.numel(), shape[0], width)
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
             _capi.check(lib.vr_lookup_backward(C.byref(lookup), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
                                                _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
         return d_table, None, d_scale, None, None
