@@ -32,62 +32,63 @@ def _row_layout(t, lead, width):
 
 
 def _arguments(table, ids, scale, width, out_dtype):
-    """(VrLookup, what has to stay alive)"""
+    """(VrLookup, the tensors behind its pointers: table, ids, scales or None)"""
     table, stride = _row_layout(table, 1, width)
     ids = ids.contiguous()
-    by_row = isinstance(scale, torch.Tensor)
-    s = scale.contiguous() if by_row else None
-    return _capi.VrLookup(_capi.ptr(table), _capi.ptr(ids), _capi.ptr(s), ids.numel(), table.shape[0], width, stride,
-                          _capi.VR_DTYPES[table.dtype], _capi.VR_DTYPES[out_dtype], int(ids.dtype == torch.int64),
-                          1.0 if by_row else scale), (table, ids, s)
+    rows = None
+    if isinstance(scale, torch.Tensor):
+        rows, scale = scale.contiguous(), 1.0
+    return _capi.VrLookup(_capi.ptr(table), _capi.ptr(ids), _capi.ptr(rows), ids.numel(), table.shape[0], width, stride,
+                          _capi.VR_DTYPES[table.dtype], _capi.VR_DTYPES[out_dtype], ids.dtype == torch.int64, scale), table, ids, rows
 
 
-def _forward(table, ids, scale, width, dtype):
-    device = table.device
+def _forward(arguments, shape, dtype, device):
     with _capi.on(device):
-        out = torch.empty(ids.shape + table.shape[1:], dtype=dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=device)
         if out.numel():
-            lookup, keep = _arguments(table, ids, scale, width, dtype)
-            _capi.check(_capi.load().vr_lookup_forward(C.byref(lookup), out.data_ptr(),
-                                                       _capi.stream_of(device)))
+            _capi.check(_capi.load().vr_lookup_forward(C.byref(arguments), out.data_ptr(), _capi.stream_of(device)))
     return out
+
+
+def _backward(ctx, g):
+    table, ids, scale = ctx.saved_tensors         # (what ctx.arguments points at)
+    arguments, shape, dtype, device = ctx.arguments, ctx.shape, ctx.dtype, g.device
+    want_table, _, want_scale = ctx.needs_input_grad[:3]
+    with _capi.on(device):
+        d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
+        d_scale = torch.empty(ctx.ids_shape, dtype=torch.float32, device=device) if want_scale else None
+        if arguments.width == 0 or arguments.n == 0:
+            return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
+        g, g_stride = _row_layout(g, len(ctx.ids_shape), arguments.width)
+        if table is None:                         # (a stand-in with the table's sizes: no value of it is read)
+            arguments.table, arguments.table_stride = _capi.ptr(d_table), arguments.width
+        lib = _capi.load()
+        scratch, nbytes = None, 0
+        if want_table:
+            nbytes = lib.vr_lookup_scratch_bytes(arguments.n, arguments.rows, arguments.width)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _capi.check(lib.vr_lookup_backward(C.byref(arguments), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
+                                           _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
+    return d_table, None, d_scale, None, None
 
 
 class _Lookup(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, ids, scale, width, dtype):
-        out = _forward(table, ids, scale, width, dtype)
-        ctx.scale, ctx.width, ctx.dtype = None if isinstance(scale, torch.Tensor) else scale, width, dtype
-        ctx.like = table.shape, table.dtype, table.device
+        ctx.arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
+        ctx.shape, ctx.dtype, ctx.ids_shape = table.shape, table.dtype, ids.shape
         # (the table's values are only needed for the gradient of the scales)
-        ctx.save_for_backward(table if ctx.needs_input_grad[2] else None, ids, scale if ctx.scale is None else None)
-        return out
+        ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, flat, scales)
+        return _forward(ctx.arguments, ids.shape + table.shape[1:], dtype, table.device)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        table, ids, scale = ctx.saved_tensors
-        shape, dtype, device = ctx.like
-        width = ctx.width
-        want_table, want_scale = ctx.needs_input_grad[0], ctx.needs_input_grad[2]
-        with _capi.on(device):
-            d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
-            d_scale = torch.empty(ids.shape, dtype=torch.float32, device=device) if want_scale else None
-            if width == 0 or ids.numel() == 0:
-                return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
-            g, g_stride = _row_layout(g, ids.dim(), width)
-            if table is None:                     # (a stand-in with the table's sizes: no value of it is read)
-                table = d_table
-            lookup, keep = _arguments(table, ids, ctx.scale if scale is None else scale, width, ctx.dtype)
-            lib = _capi.load()
-            scratch, nbytes = None, 0
-            if want_table:
-                nbytes = lib.vr_lookup_scratch_bytes(ids.numel(), shape[0], width)
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-            _capi.check(lib.vr_lookup_backward(C.byref(lookup), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
-                                               _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
-        return d_table, None, d_scale, None, None
+        # (grad mode is on where the caller asked for a graph of the gradients, which are not differentiable again)
+        return _backward_once(ctx, g) if torch.is_grad_enabled() else _backward(ctx, g)
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def lookup(table, ids, scale=None, dtype=None):
@@ -125,4 +126,5 @@ def lookup(table, ids, scale=None, dtype=None):
         raise ValueError("rows of more than 2^24 values")
     if torch.is_grad_enabled() and (table.requires_grad or (isinstance(scale, torch.Tensor) and scale.requires_grad)):
         return _Lookup.apply(table, ids, scale, width, dtype)
-    return _forward(table, ids, scale, width, dtype)
+    arguments, *keep = _arguments(table, ids, scale, width, dtype)
+    return _forward(arguments, ids.shape + table.shape[1:], dtype, device)
