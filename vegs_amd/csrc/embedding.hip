@@ -111,23 +111,6 @@ __global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict
     }
 }
 
-// First launch of the table's gradient: the sort's keys -- the row, or `rows` for "no row" (sorted behind every row) -- and its values,
-// the entries; workgroups behind those clear the gradient, of which only the rows with entries are written later.
-__global__ void __launch_bounds__(256)
-k_lookup_keys(LookupArgs a, uint32_t* __restrict__ key, uint32_t* __restrict__ val, int key_blocks, char* __restrict__ zero,
-              long zero_bytes)
-{
-    if ((int)blockIdx.x < key_blocks) {
-        const long i = (long)blockIdx.x * 256 + threadIdx.x;
-        if (i >= a.n) return;
-        const long row = row_of(a, i);
-        key[i] = row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
-        val[i] = (uint32_t)i;
-        return;
-    }
-    zero_fill(zero, zero_bytes, (long)(blockIdx.x - key_blocks) * 256 + threadIdx.x, (long)(gridDim.x - key_blocks) * 256);
-}
-
 constexpr uint32_t NO_ENTRY = 0xffffffffu;            // behind every row and behind "no row"
 
 // ---- the sort of few entries by one workgroup: all of them stay in LDS through the passes (stable, 8 bits each).
@@ -230,6 +213,163 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
     }
 }
 
+// ---- the sort of many entries: stable, least significant digit first, digits of up to 8 bits; a pass is a histogram per block of
+// SORT_BLOCK entries, the sums over the blocks of each digit, and the scatter.  The first pass takes its keys from the ids, and its
+// histogram's launch clears the table's gradient in further workgroups.  The scales travel with the entries: gathered afterwards, every
+// one of them would fetch a line of its own (2 M entries: 23 us of the sums' 162, 5 us here).
+constexpr int SORT_BLOCK = 4096, PASS_THREADS = 512, PASS_WAVES = PASS_THREADS / 64, PASS_ITEMS = SORT_BLOCK / PASS_THREADS;
+
+struct PassArgs {
+    const uint32_t *key, *val;      // NULL in the first pass: from the ids
+    const float* scale;             // NULL: none travel
+    uint32_t *key_out, *val_out;
+    float* scale_out;
+    uint32_t *hist, *totals;        // [digits][blocks] counts, then their exclusive sums; [digits]
+    int blocks, shift, bits;
+};
+
+__device__ __forceinline__ uint32_t pass_key(const LookupArgs& a, const PassArgs& p, long i)
+{
+    if (p.key) return p.key[i];
+    const long row = row_of(a, i);
+    return row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
+}
+
+__global__ void __launch_bounds__(PASS_THREADS) k_sort_hist(LookupArgs a, PassArgs p, char* __restrict__ zero, long zero_bytes)
+{
+    __shared__ uint32_t count[256];
+    if ((int)blockIdx.x >= p.blocks) {
+        zero_fill(zero, zero_bytes, (long)(blockIdx.x - p.blocks) * PASS_THREADS + threadIdx.x, (long)(gridDim.x - p.blocks) * PASS_THREADS);
+        return;
+    }
+    const uint32_t mask = (1u << p.bits) - 1u;
+    if (threadIdx.x < 256) count[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t key[PASS_ITEMS];
+#pragma unroll
+    for (int x = 0; x < PASS_ITEMS; ++x) {
+        const long i = (long)blockIdx.x * SORT_BLOCK + x * PASS_THREADS + threadIdx.x;
+        key[x] = i < a.n ? pass_key(a, p, i) : 0u;
+    }
+#pragma unroll
+    for (int x = 0; x < PASS_ITEMS; ++x) {
+        const long i = (long)blockIdx.x * SORT_BLOCK + x * PASS_THREADS + threadIdx.x;
+        if (i < a.n) atomicAdd(&count[(key[x] >> p.shift) & mask], 1u);        // (counts: their order does not matter)
+    }
+    __syncthreads();
+    if (threadIdx.x <= mask) p.hist[(size_t)threadIdx.x * p.blocks + blockIdx.x] = count[threadIdx.x];
+}
+
+// one workgroup per digit: the exclusive sums of its counts over the blocks, in place, and their total
+__global__ void __launch_bounds__(256) k_sort_sums(PassArgs p)
+{
+    __shared__ uint32_t wave_sum[4];
+    uint32_t* h = p.hist + (size_t)blockIdx.x * p.blocks;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (int first = 0; first < p.blocks; first += 256) {
+        const int i = first + threadIdx.x;
+        const uint32_t c = i < p.blocks ? h[i] : 0u;
+        uint32_t incl = c;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)incl, d, 64);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 63) wave_sum[w] = incl;
+        __syncthreads();
+        uint32_t base = carry;
+        for (int k = 0; k < w; ++k) base += wave_sum[k];
+        if (i < p.blocks) h[i] = base + incl - c;
+        carry += wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
+}
+
+// The block's entries are put in the order of their digits in LDS first, so that what goes to one digit leaves as one piece.
+__global__ void __launch_bounds__(PASS_THREADS) k_sort_scatter(LookupArgs a, PassArgs p)
+{
+    __shared__ uint32_t cnt[PASS_WAVES][256], local[256], global[256], wave_sum[2][4];
+    __shared__ uint32_t skey[SORT_BLOCK], sval[SORT_BLOCK];
+    __shared__ float sscale[SORT_BLOCK];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * PASS_ITEMS) + lane;
+    const long block = (long)blockIdx.x * SORT_BLOCK;
+    const int n = (int)(a.n - block < SORT_BLOCK ? a.n - block : SORT_BLOCK);
+    const uint32_t mask = (1u << p.bits) - 1u;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    for (int d = threadIdx.x; d < PASS_WAVES * 256; d += PASS_THREADS) (&cnt[0][0])[d] = 0;
+    uint32_t key[PASS_ITEMS], val[PASS_ITEMS], rank[PASS_ITEMS];
+    float scale[PASS_ITEMS];
+#pragma unroll
+    for (int x = 0; x < PASS_ITEMS; ++x) {
+        const int i = first + 64 * x;
+        const bool in = i < n;
+        key[x] = in ? pass_key(a, p, block + i) : NO_ENTRY;
+        val[x] = in && p.val ? p.val[block + i] : (uint32_t)(block + i);
+        scale[x] = in && p.scale ? p.scale[block + i] : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < PASS_ITEMS; ++x) {
+        const bool in = first + 64 * x < n;
+        const uint32_t d = (key[x] >> p.shift) & mask;
+        unsigned long long same = __ballot(in);
+        for (int b = 0; b < p.bits; ++b) {
+            const unsigned long long on = __ballot((d >> b) & 1u);
+            same &= ((d >> b) & 1u) ? on : ~on;
+        }
+        const uint32_t prior = cnt[w][d];
+        rank[x] = prior + (uint32_t)__popcll(same & before);
+        __builtin_amdgcn_wave_barrier();
+        if (in && (same & before) == 0) cnt[w][d] = prior + (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // per digit: where the waves' entries begin in the block, and where the block's begin among all
+    uint32_t total = 0, incl = 0, all = 0, all_incl = 0;
+    if (threadIdx.x < 256) {
+        for (int k = 0; k < PASS_WAVES; ++k) {
+            const uint32_t c = cnt[k][threadIdx.x];
+            cnt[k][threadIdx.x] = total;
+            total += c;
+        }
+        all = threadIdx.x <= mask ? p.totals[threadIdx.x] : 0u;
+        incl = total;
+        all_incl = all;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)incl, d, 64), q = (uint32_t)__shfl_up((int)all_incl, d, 64);
+            if (lane >= d) { incl += o; all_incl += q; }
+        }
+        if (lane == 63) { wave_sum[0][w] = incl; wave_sum[1][w] = all_incl; }
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) {
+        uint32_t l = incl - total, g = all_incl - all;
+        for (int k = 0; k < w; ++k) { l += wave_sum[0][k]; g += wave_sum[1][k]; }
+        local[threadIdx.x] = l;
+        global[threadIdx.x] = threadIdx.x <= mask ? g + p.hist[(size_t)threadIdx.x * p.blocks + blockIdx.x] : 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < PASS_ITEMS; ++x) {
+        if (first + 64 * x < n) {
+            const uint32_t d = (key[x] >> p.shift) & mask, at = local[d] + cnt[w][d] + rank[x];
+            skey[at] = key[x];
+            sval[at] = val[x];
+            sscale[at] = scale[x];
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < n; j += PASS_THREADS) {
+        const uint32_t k = skey[j], d = (k >> p.shift) & mask, to = global[d] + ((uint32_t)j - local[d]);
+        p.key_out[to] = k;
+        p.val_out[to] = sval[j];
+        if (p.scale) p.scale_out[to] = sscale[j];
+    }
+}
+
 // ---- the sums of the table's gradient over the sorted entries.
 //
 // Split by ENTRIES, not by rows, so that a row hit a million times costs what a million rows hit once do: a group of G lanes
@@ -244,6 +384,7 @@ constexpr int UNROLL = 8;
 
 struct SumArgs {
     const uint32_t *key, *val;
+    const float* scales;          // in the entries' sorted order; NULL: row_scale by entry
     const void* grad;
     long grad_stride;
     void* d_table;
@@ -295,7 +436,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 #pragma unroll
         for (int x = 0; x < UNROLL; ++x) {
             const bool there = key[x] < rows;
-            s[x] = there && a.row_scale ? a.row_scale[val[x]] : 1.0f;
+            s[x] = q.scales ? q.scales[j + x] : there && a.row_scale ? a.row_scale[val[x]] : 1.0f;     // (padded as the keys)
             g[x] = load_once<TO, V>(grad + (there ? (long)val[x] * q.grad_stride : 0));
             if (DSCALE) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (there ? (long)key[x] * a.table_stride : 0));
         }
@@ -395,14 +536,31 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         const unsigned long long mask = __ballot(owner);           // (one wave: JOIN_CHUNKS is 64)
         if (threadIdx.x == 0) count = __popcll(mask);
         if (owner) {
-            // the last chunk whose first entry is of this row: doubling steps, then halving ones
-            long lo = c + 1, step = 1;
-            while (lo + step < chunks && q.key[(lo + step) * q.chunk] == k) { lo += step; step <<= 1; }
-            for (; step > 0; step >>= 1)
-                if (lo + step < chunks && q.key[(lo + step) * q.chunk] == k) lo += step;
             const int at = __popcll(mask & ((1ull << threadIdx.x) - 1ull));
-            from[at] = c; upto[at] = lo; row[at] = k;
+            from[at] = c; row[at] = k;
         }
+    }
+    __syncthreads();
+    // the last chunk whose first entry is of the row, a wave per row: chunks 1, 2, 4, ... further on at once, then 64 in between
+    for (int o = threadIdx.x >> 6; o < count; o += JOIN_THREADS / 64) {
+        const long base = from[o] + 1;
+        const uint32_t k = row[o];
+        const int at = threadIdx.x & 63;
+        long lo = 0, x = at < 31 ? 1l << at : chunks;
+        unsigned long long off = ~__ballot(base + x < chunks && q.key[(base + (base + x < chunks ? x : 0)) * q.chunk] == k);
+        const int t = __ffsll(off) - 1;                            // (lane 63 is always off)
+        lo = t == 0 ? 0 : 1l << (t - 1);
+        long hi = 1l << t;                                         // not of the row, or behind the last chunk
+        if (hi > chunks - base) hi = chunks - base;
+        while (hi - lo > 1) {
+            const long step = (hi - lo + 63) / 64;
+            x = lo + (at + 1) * step;
+            off = ~__ballot(x < hi && q.key[(base + (x < hi ? x : lo)) * q.chunk] == k);
+            const int more = off == 0 ? 64 : __ffsll(off) - 1;
+            lo += more * step;
+            if (lo + step < hi) hi = lo + step;
+        }
+        if (at == 0) upto[o] = base + lo;
     }
     __syncthreads();
     const float* slots = q.slots + col;
@@ -703,19 +861,29 @@ extern "C" int vr_lookup_forward(const VrLookup* lookup, void* out, void* stream
     return by_type<Forward>(lookup, a, out, (hipStream_t)stream);
 }
 
-// scratch: two pairs of key and value arrays, the sort's own, and the slots of the chunks (a chunk has UNROLL entries at
-// least; the tiling of the wider type has the shorter chunks)
-static size_t slots_bytes(int64_t n, int64_t width)
+// scratch: two sets of keys, values and scales, the sort's counts, and the slots of the chunks
+struct Scratch {
+    size_t array, arrays, hist, slots;      // bytes of one array, of all, of the counts and totals, of the slots
+    int blocks;
+};
+static Scratch scratch_of(int64_t n, int64_t width)
 {
+    Scratch s;
+    s.array = align_up((size_t)n * 4, 256);         // (whole chunks of 64 entries)
+    s.blocks = (int)((n + SORT_BLOCK - 1) / SORT_BLOCK);
+    s.arrays = n <= SORT_SMALL ? 2 * s.array : 6 * s.array;
+    s.hist = n <= SORT_SMALL ? 0 : align_up(256 * (size_t)s.blocks * 4 + 256 * 4, 256);
     const long chunks = tiling(n, width, 4).chunks > tiling(n, width, 8).chunks ? tiling(n, width, 4).chunks : tiling(n, width, 8).chunks;
-    return align_up((size_t)chunks * 2 * (size_t)width * sizeof(float), 256);
+    s.slots = align_up((size_t)chunks * 2 * (size_t)width * sizeof(float), 256);
+    return s;
 }
 
 extern "C" int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width)
 {
     if (n < 0 || n >= (1ll << 30) || rows < 0 || rows >= 0x7fffffffll || width < 1 || width > (1 << 24)) return 0;
     if (n <= SMALL) return 0;
-    return (int64_t)(4 * align_up((size_t)n * 4, 256) + align_up(sort_pairs_scratch_bytes((long)n), 256) + slots_bytes(n, width));
+    const Scratch s = scratch_of(n, width);
+    return (int64_t)(s.arrays + s.hist + s.slots);
 }
 
 extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int64_t grad_stride, void* d_table, float* d_row_scale,
@@ -732,31 +900,49 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
     if (a.rows == 0) d_table = nullptr;
     if (!d_table && (!d_row_scale || a.n == 0)) return VR_OK;
     hipStream_t s = (hipStream_t)stream;
-    SumArgs q{nullptr, nullptr, grad, (long)grad_stride, d_table, d_row_scale, nullptr, 0, 0};
+    SumArgs q{nullptr, nullptr, nullptr, grad, (long)grad_stride, d_table, d_row_scale, nullptr, 0, 0};
     if (d_table && a.n > SMALL) {
-        const size_t arr = align_up((size_t)a.n * 4, 256);
+        const Scratch sc = scratch_of(a.n, a.width);
         char* base = (char*)scratch;
-        uint32_t *k0 = (uint32_t*)base, *v0 = (uint32_t*)(base + arr), *k1 = (uint32_t*)(base + 2 * arr), *v1 = (uint32_t*)(base + 3 * arr);
+        uint32_t *key[2], *val[2];
+        float* scale[2];
+        for (int k = 0; k < 2; ++k) {
+            key[k] = (uint32_t*)(base + (a.n <= SORT_SMALL ? 0 : k) * 3 * sc.array);
+            val[k] = key[k] + sc.array / 4;
+            scale[k] = (float*)(val[k] + sc.array / 4);
+        }
+        q.slots = (float*)(base + sc.arrays + sc.hist);
         const long zero_bytes = a.rows * a.width * (long)t_element, zero_blocks = (zero_bytes + 16383) / 16384;
+        const int bits = key_bits(a.rows);
         if (a.n <= SORT_SMALL) {
             const dim3 grid(1 + (unsigned)(zero_blocks < 1024 ? zero_blocks : 1024));
-            const int bits = key_bits(a.rows);
-            if (a.n <= 4 * SORT_THREADS) hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
-            else hipLaunchKernelGGL(k_lookup_sort<16>, grid, dim3(SORT_THREADS), 0, s, a, k0, v0, bits, (char*)d_table, zero_bytes);
+            if (a.n <= 4 * SORT_THREADS)
+                hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, key[0], val[0], bits, (char*)d_table, zero_bytes);
+            else
+                hipLaunchKernelGGL(k_lookup_sort<16>, grid, dim3(SORT_THREADS), 0, s, a, key[0], val[0], bits, (char*)d_table, zero_bytes);
             VR_KERNEL_CHECK("lookup_sort", s, false);
-            q.key = k0;
-            q.val = v0;
+            q.key = key[0];
+            q.val = val[0];
         } else {
-            const int key_blocks = cdiv(a.n, 256);
-            hipLaunchKernelGGL(k_lookup_keys, dim3(key_blocks + (unsigned)(zero_blocks < 4096 ? zero_blocks : 4096)), dim3(256), 0, s, a, k0,
-                               v0, key_blocks, (char*)d_table, zero_bytes);
-            VR_KERNEL_CHECK("lookup_keys", s, false);
-            int where = 0;
-            if (int rc = launch_sort_pairs(k0, v0, k1, v1, a.n, 0u, key_bits(a.rows), base + 4 * arr, s, false, &where)) return rc;
-            q.key = where ? k1 : k0;
-            q.val = where ? v1 : v0;
+            const int passes = (bits + 7) / 8;
+            PassArgs p{nullptr, nullptr, a.row_scale, nullptr, nullptr, nullptr, (uint32_t*)(base + sc.arrays), nullptr, sc.blocks, 0, 0};
+            p.totals = p.hist + 256 * (size_t)sc.blocks;
+            for (int pass = 0, to = 0; pass < passes; ++pass, to ^= 1) {
+                p.bits = (bits - p.shift + passes - pass - 1) / (passes - pass);          // as even as they get
+                p.key_out = key[to]; p.val_out = val[to]; p.scale_out = scale[to];
+                const unsigned zeros = pass > 0 ? 0 : (unsigned)(zero_blocks < 2048 ? zero_blocks : 2048);
+                hipLaunchKernelGGL(k_sort_hist, dim3(sc.blocks + zeros), dim3(PASS_THREADS), 0, s, a, p, (char*)d_table, zero_bytes);
+                hipLaunchKernelGGL(k_sort_sums, dim3(1u << p.bits), dim3(256), 0, s, p);
+                hipLaunchKernelGGL(k_sort_scatter, dim3(sc.blocks), dim3(PASS_THREADS), 0, s, a, p);
+                VR_KERNEL_CHECK("lookup_sort", s, false);
+                p.key = p.key_out; p.val = p.val_out;
+                if (p.scale) p.scale = p.scale_out;
+                p.shift += p.bits;
+            }
+            q.key = p.key;
+            q.val = p.val;
+            q.scales = p.scale;
         }
-        q.slots = (float*)(base + 4 * arr + align_up(sort_pairs_scratch_bytes(a.n), 256));
     }
     return by_type<Backward>(lookup, a, q, s);
 }
