@@ -217,7 +217,7 @@ k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict
 // SORT_BLOCK entries, the sums over the blocks of each digit, and the scatter.  The first pass takes its keys from the ids, and its
 // histogram's launch clears the table's gradient in further workgroups.  The scales travel with the entries: gathered afterwards, every
 // one of them would fetch a line of its own (2 M entries: 23 us of the sums' 162, 5 us here).
-constexpr int SORT_BLOCK = 4096, PASS_THREADS = 512, PASS_WAVES = PASS_THREADS / 64, PASS_ITEMS = SORT_BLOCK / PASS_THREADS;
+constexpr int SORT_BLOCK = 4096, PASS_THREADS = 1024, PASS_WAVES = PASS_THREADS / 64, PASS_ITEMS = SORT_BLOCK / PASS_THREADS;
 
 struct PassArgs {
     const uint32_t *key, *val;      // NULL in the first pass: from the ids
@@ -397,6 +397,7 @@ struct SumArgs {
 template <typename TT, typename TO, int V, bool DSCALE>
 __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 {
+    constexpr int U = UNROLL, U_SHIFT = 3;
     const int G = 1 << q.g_shift, lane = threadIdx.x & (G - 1);
     const long chunk = ((long)blockIdx.x * 256 + threadIdx.x) >> q.g_shift;
     const long first = chunk * q.chunk, last = first + q.chunk < a.n ? first + q.chunk : a.n;
@@ -410,46 +411,42 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
     const TT* table = reinterpret_cast<const TT*>(a.table) + col;
     TT* d_table = reinterpret_cast<TT*>(q.d_table) + col;
     float* slot = q.slots + (2 * chunk) * a.width + col;
-    // (the arrays are padded to whole chunks: the loads of keys and entries need no bounds, what lies behind `last` is masked)
-    uint4 next_key[UNROLL / 4], next_val[UNROLL / 4];
-#pragma unroll
-    for (int x = 0; x < UNROLL / 4; ++x) {
-        next_key[x] = reinterpret_cast<const uint4*>(q.key + first)[x];
-        next_val[x] = reinterpret_cast<const uint4*>(q.val + first)[x];
-    }
     uint32_t cur = q.key[first];
     bool came_in = first > 0 && q.key[first - 1] == cur;
+    Pack<TT, V> t_cur;
+    if (DSCALE && cur < rows) t_cur = *reinterpret_cast<const Pack<TT, V>*>(table + (long)cur * a.table_stride);
     float acc[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-    for (long j = first; j < last; j += UNROLL) {
-        uint32_t key[UNROLL], val[UNROLL];
+    for (long j = first; j < last; j += U) {
+        // (the arrays are padded to whole chunks: the loads need no bounds, what lies behind `last` is masked)
+        uint4 k4[U / 4], v4[U / 4];
 #pragma unroll
-        for (int x = 0; x < UNROLL; ++x) {
-            const bool in = j + x < last;
-            key[x] = in ? (&next_key[x / 4].x)[x % 4] : NO_ENTRY;
-            val[x] = in ? (&next_val[x / 4].x)[x % 4] : 0u;
+        for (int x = 0; x < U / 4; ++x) {
+            k4[x] = reinterpret_cast<const uint4*>(q.key + j)[x];
+            v4[x] = reinterpret_cast<const uint4*>(q.val + j)[x];
         }
-        Pack<TO, V> g[UNROLL];
-        Pack<TT, V> t[UNROLL];
-        float s[UNROLL];
+        uint32_t key[U], val[U];
 #pragma unroll
-        for (int x = 0; x < UNROLL; ++x) {
+        for (int x = 0; x < U; ++x) {
+            const bool in = j + x < last;
+            key[x] = in ? (&k4[x / 4].x)[x % 4] : NO_ENTRY;
+            val[x] = in ? (&v4[x / 4].x)[x % 4] : 0u;
+        }
+        Pack<TO, V> g[U];
+        Pack<TT, V> t[U];
+        float s[U];
+#pragma unroll
+        for (int x = 0; x < U; ++x) {
             const bool there = key[x] < rows;
             s[x] = q.scales ? q.scales[j + x] : there && a.row_scale ? a.row_scale[val[x]] : 1.0f;     // (padded as the keys)
             g[x] = load_once<TO, V>(grad + (there ? (long)val[x] * q.grad_stride : 0));
-            if (DSCALE) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (there ? (long)key[x] * a.table_stride : 0));
+            // (a row of the table is read where it begins among the entries, not again for each of them)
+            if (DSCALE && there && key[x] != (x == 0 ? cur : key[x - 1])) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (long)key[x] * a.table_stride);
         }
-        if (j + UNROLL < last) {               // the next ones travel while these rows are added
+        float dot[U];
 #pragma unroll
-            for (int x = 0; x < UNROLL / 4; ++x) {
-                next_key[x] = reinterpret_cast<const uint4*>(q.key + j + UNROLL)[x];
-                next_val[x] = reinterpret_cast<const uint4*>(q.val + j + UNROLL)[x];
-            }
-        }
-        float dot[UNROLL];
-#pragma unroll
-        for (int x = 0; x < UNROLL; ++x) {
+        for (int x = 0; x < U; ++x) {
             if (key[x] != cur && key[x] != NO_ENTRY) {
                 if (live && cur < rows) {
                     if (came_in) store_row<float, V>(slot, acc);
@@ -457,6 +454,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
                 }
                 came_in = false;
                 cur = key[x];
+                if (DSCALE) t_cur = t[x];
 #pragma unroll
                 for (int v = 0; v < V; ++v) acc[v] = 0.0f;
             }
@@ -467,16 +465,37 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
                 for (int v = 0; v < V; ++v) {
                     const float gv = load_f32(g[x].v + v);
                     acc[v] = fmaf(sx, gv, acc[v]);
-                    if (DSCALE && col + v >= want) dot[x] = fmaf(gv, load_f32(t[x].v + v), dot[x]);
+                    if (DSCALE && col + v >= want) dot[x] = fmaf(gv, load_f32(t_cur.v + v), dot[x]);
                 }
             }
         }
         if (DSCALE) {
+            // the group's sums of the U products.  Where it has as many lanes, half of them pass on the half of the sums
+            // that the others keep, three times, so that every eighth of the lanes ends with one sum: 8 exchanges and one store
+            // for 16 lanes where a butterfly for each sum takes 32 and eight (2 M x 45: 150 us against 155)
+            float d[U];
 #pragma unroll
-            for (int x = 0; x < UNROLL; ++x) {
-                float d = live ? dot[x] : 0.0f;
-                for (int w = G >> 1; w > 0; w >>= 1) d += __shfl_xor(d, w, 64);
-                if (lane == 0 && j + x < last) q.d_row_scale[val[x]] = a.scale * d;
+            for (int x = 0; x < U; ++x) d[x] = live ? dot[x] : 0.0f;
+            if (q.g_shift >= U_SHIFT) {
+                int w = G >> 1;
+#pragma unroll
+                for (int half = U / 2; half > 0; half >>= 1, w >>= 1) {
+                    const bool high = (lane & w) != 0;
+#pragma unroll
+                    for (int x = 0; x < half; ++x) {
+                        const float keep = high ? d[x + half] : d[x], pass = high ? d[x] : d[x + half];
+                        d[x] = keep + __shfl_xor(pass, w, 64);
+                    }
+                }
+                for (; w > 0; w >>= 1) d[0] += __shfl_xor(d[0], w, 64);
+                const int x = lane >> (q.g_shift - U_SHIFT);
+                if ((lane & ((G >> U_SHIFT) - 1)) == 0 && j + x < last) q.d_row_scale[q.val[j + x]] = a.scale * d[0];
+            } else {
+#pragma unroll
+                for (int x = 0; x < U; ++x) {
+                    for (int w = G >> 1; w > 0; w >>= 1) d[x] += __shfl_xor(d[x], w, 64);
+                    if (lane == 0 && j + x < last) q.d_row_scale[val[x]] = a.scale * d[x];
+                }
             }
         }
     }
