@@ -20,7 +20,7 @@ typedef struct VrLookup {
     const float* row_scale;  /* device [n]; NULL: ones */
     int64_t n;               /* < 2^30 */
     int64_t rows;            /* < 2^31 - 1 */
-    int64_t width;           /* 1 .. 2^24 */
+    int64_t width;           /* 1 .. 2^22 */
     int64_t table_stride;    /* >= width */
     int32_t table_dtype;     /* VrDataType */
     int32_t out_dtype;       /* VrDataType of out and grad: table_dtype, or VR_F32 */
@@ -35,7 +35,8 @@ int vr_lookup_forward(const VrLookup* lookup, void* out, void* stream);
 int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width);
 
 /* grad [n, width], rows grad_stride elements apart.  d_table [rows, width] in the table's type, every element written; NULL:
- * not wanted (scratch may be NULL then, and where no scratch is needed).  d_row_scale [n] fp32; NULL: not wanted.  Sums are fp32 (in pieces of a fixed size that are
+ * not wanted (scratch may be NULL then, and where no scratch is needed).  d_row_scale [n] fp32; NULL: not wanted
+ * (no value of the table is read then).  Sums are fp32 (in pieces of a fixed size that are
  * joined in order: the same inputs give the same bits) and rounded once. */
 int vr_lookup_backward(const VrLookup* lookup, const void* grad, int64_t grad_stride, void* d_table, float* d_row_scale,
                        void* scratch, int64_t scratch_bytes, void* stream);

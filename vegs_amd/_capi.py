@@ -248,11 +248,11 @@ def load():
     lib.vr_sh_adam_step_clipped.argtypes = [vp, i32, vp, vp, i32, C.c_int64, i32, i32, C.c_float, C.POINTER(VrShAdamTensor),
                                             C.POINTER(VrShAdamTensor), C.c_double, C.c_double, C.c_double, vp, C.c_float, vp]
     lib.vr_lookup_forward.restype = C.c_int
-    lib.vr_lookup_forward.argtypes = [C.POINTER(VrLookup), vp, vp]
+    lib.vr_lookup_forward.argtypes = [vp, vp, vp]
     lib.vr_lookup_scratch_bytes.restype = C.c_int64
     lib.vr_lookup_scratch_bytes.argtypes = [C.c_int64] * 3
     lib.vr_lookup_backward.restype = C.c_int
-    lib.vr_lookup_backward.argtypes = [C.POINTER(VrLookup), vp, C.c_int64, vp, vp, vp, C.c_int64, vp]
+    lib.vr_lookup_backward.argtypes = [vp, vp, C.c_int64, vp, vp, vp, C.c_int64, vp]
     lib.vr_instances_forward.restype = C.c_int
     lib.vr_instances_forward.argtypes = [C.POINTER(VrInstance), i32, vp, vp, vp, vp]
     lib.vr_instances_backward.restype = C.c_int

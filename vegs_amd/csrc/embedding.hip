@@ -781,9 +781,9 @@ static Tiling tiling(int64_t n, int64_t width, int v_full)
 static int check_lookup(const VrLookup* l, LookupArgs& a)
 {
     if (!l) { set_error("lookup: arguments are required"); return VR_ERR_INVALID_ARGUMENT; }
-    if (l->n < 0 || l->n >= (1ll << 30) || l->rows < 0 || l->rows >= 0x7fffffffll || l->width < 1 || l->width > (1 << 24) ||
+    if (l->n < 0 || l->n >= (1ll << 30) || l->rows < 0 || l->rows >= 0x7fffffffll || l->width < 1 || l->width > (1 << 22) ||
         l->table_stride < l->width || l->table_stride > (1ll << 40))
-        { set_error("lookup: need 0 <= n < 2^30, 0 <= rows < 2^31 - 1, 1 <= width <= 2^24, table_stride >= width"); return VR_ERR_INVALID_ARGUMENT; }
+        { set_error("lookup: need 0 <= n < 2^30, 0 <= rows < 2^31 - 1, 1 <= width <= 2^22, table_stride >= width"); return VR_ERR_INVALID_ARGUMENT; }
     if (l->table_dtype < VR_F32 || l->table_dtype > VR_F16 || (l->out_dtype != l->table_dtype && l->out_dtype != VR_F32))
         { set_error("lookup: the output has the table's type or fp32"); return VR_ERR_INVALID_ARGUMENT; }
     const uintptr_t element = l->table_dtype == VR_F32 ? 4 : 2, id = l->ids_64 ? 8 : 4;
@@ -899,7 +899,7 @@ static Scratch scratch_of(int64_t n, int64_t width)
 
 extern "C" int64_t vr_lookup_scratch_bytes(int64_t n, int64_t rows, int64_t width)
 {
-    if (n < 0 || n >= (1ll << 30) || rows < 0 || rows >= 0x7fffffffll || width < 1 || width > (1 << 24)) return 0;
+    if (n < 0 || n >= (1ll << 30) || rows < 0 || rows >= 0x7fffffffll || width < 1 || width > (1 << 22)) return 0;
     if (n <= SMALL) return 0;
     const Scratch s = scratch_of(n, width);
     return (int64_t)(s.arrays + s.hist + s.slots);

@@ -8,13 +8,15 @@ one id per Gaussian; the result IS the f_rest input of the rasterizer, next to i
 pose corrections by frame.  The table's gradient is dense, in the table's type, so vegs_amd.optim.Adam, grad_norm and the
 exchanges of vegs_amd.dist take it like any other.  GPU tensors only; there is no CPU path.
 """
-import ctypes as C
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
+
+_ID_TYPES = (torch.int32, torch.int64)
 
 
 def _row_layout(t, lead, width):
@@ -31,45 +33,59 @@ def _row_layout(t, lead, width):
     return t.contiguous(), width
 
 
-def _arguments(table, ids, scale, width, out_dtype):
-    """(VrLookup, the tensors behind its pointers: table, ids, scales or None)"""
-    table, stride = _row_layout(table, 1, width)
-    ids = ids.contiguous()
-    rows = None
+_LOOKUP = struct.Struct("3Q4q3if")           # VrLookup
+
+
+def _arguments(table, ids, scale, width, dtype):
+    """(VrLookup as packed bytes, the tensors behind its pointers: table, ids, scales or None)"""
+    stride, rows, at = width, None, 0
+    if not table.is_contiguous():
+        table, stride = _row_layout(table, 1, width)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     if isinstance(scale, torch.Tensor):
         rows, scale = scale.contiguous(), 1.0
-    return _capi.VrLookup(_capi.ptr(table), _capi.ptr(ids), _capi.ptr(rows), ids.numel(), table.shape[0], width, stride,
-                          _capi.VR_DTYPES[table.dtype], _capi.VR_DTYPES[out_dtype], ids.dtype == torch.int64, scale), table, ids, rows
+        at = rows.data_ptr()
+    kinds = _capi.VR_DTYPES
+    return _LOOKUP.pack(table.data_ptr(), ids.data_ptr(), at, ids.numel(), table.shape[0], width, stride, kinds[table.dtype],
+                        kinds[dtype], ids.dtype == torch.int64, scale), table, ids, rows
 
 
 def _forward(arguments, shape, dtype, device):
-    with _capi.on(device):
-        out = torch.empty(shape, dtype=dtype, device=device)
-        if out.numel():
-            _capi.check(_capi.load().vr_lookup_forward(C.byref(arguments), out.data_ptr(), _capi.stream_of(device)))
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _forward(arguments, shape, dtype, device)
+    out = torch.empty(shape, dtype=dtype, device=device)
+    if out.numel():
+        _capi.check(_capi.load().vr_lookup_forward(arguments, out.data_ptr(), _capi.stream_of(device)))
     return out
 
 
 def _backward(ctx, g):
-    table, ids, scale = ctx.saved_tensors         # (what ctx.arguments points at)
-    arguments, shape, dtype, device = ctx.arguments, ctx.shape, ctx.dtype, g.device
-    want_table, _, want_scale = ctx.needs_input_grad[:3]
+    keep = ctx.saved_tensors                      # (what ctx.arguments points at, as far as it is read)
+    arguments, shape, dtype, n, width = ctx.arguments, ctx.shape, ctx.dtype, ctx.n, ctx.width
+    want_table, _, want_scale, _, _ = ctx.needs_input_grad
+    device = g.device
     with _capi.on(device):
         d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
         d_scale = torch.empty(ctx.ids_shape, dtype=torch.float32, device=device) if want_scale else None
-        if arguments.width == 0 or arguments.n == 0:
+        if width == 0 or n == 0:
             return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
-        g, g_stride = _row_layout(g, len(ctx.ids_shape), arguments.width)
-        if table is None:                         # (a stand-in with the table's sizes: no value of it is read)
-            arguments.table, arguments.table_stride = _capi.ptr(d_table), arguments.width
+        stride = width
+        if not g.is_contiguous():
+            g, stride = _row_layout(g, len(ctx.ids_shape), width)
         lib = _capi.load()
-        scratch, nbytes = None, 0
-        if want_table:
-            nbytes = lib.vr_lookup_scratch_bytes(arguments.n, arguments.rows, arguments.width)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _capi.check(lib.vr_lookup_backward(C.byref(arguments), g.data_ptr(), g_stride, _capi.ptr(d_table), _capi.ptr(d_scale),
+        scratch = None
+        nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width) if want_table else 0
+        if nbytes:
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _capi.check(lib.vr_lookup_backward(arguments, g.data_ptr(), stride, _capi.ptr(d_table), _capi.ptr(d_scale),
                                            _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
     return d_table, None, d_scale, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _Lookup(torch.autograd.Function):
@@ -77,8 +93,8 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, width, dtype):
         ctx.arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
-        ctx.shape, ctx.dtype, ctx.ids_shape = table.shape, table.dtype, ids.shape
-        # (the table's values are only needed for the gradient of the scales)
+        ctx.shape, ctx.dtype, ctx.ids_shape, ctx.n, ctx.width = table.shape, table.dtype, ids.shape, ids.numel(), width
+        # (the table's values are only read again for the gradient of the scales)
         ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, flat, scales)
         return _forward(ctx.arguments, ids.shape + table.shape[1:], dtype, table.device)
 
@@ -88,9 +104,6 @@ class _Lookup(torch.autograd.Function):
         return _backward_once(ctx, g) if torch.is_grad_enabled() else _backward(ctx, g)
 
 
-_backward_once = once_differentiable(_backward)
-
-
 def lookup(table, ids, scale=None, dtype=None):
     """scale * table[ids]: [*ids.shape, *table.shape[1:]], differentiable with respect to `table` and to a `scale` tensor.
 
@@ -98,33 +111,34 @@ def lookup(table, ids, scale=None, dtype=None):
     convention -- means "no row": zeros, and no gradient whatever stands in its place.  scale: a number, or a float32
     tensor shaped like ids.  dtype: of the result, the table's (default) or float32.
 
-    The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in their order, in
-    float32, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same bits every time."""
+    The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in float32, in an order
+    that the sizes fix, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same
+    bits every time."""
     if not isinstance(table, torch.Tensor) or not table.is_cuda:
         raise ValueError("table must be a GPU tensor (there is no CPU path)")
-    if table.dim() < 1 or table.dtype not in _capi.VR_DTYPES or table.layout != torch.strided:
-        raise ValueError(f"table must be a dense float32, bfloat16 or float16 tensor [K, ...] (got {table.dtype} {tuple(table.shape)})")
-    device = table.device
-    if not isinstance(ids, torch.Tensor) or ids.device != device or ids.dtype not in (torch.int32, torch.int64):
+    shape, kind, device = table.shape, table.dtype, table.device
+    if not shape or kind not in _capi.VR_DTYPES or table.layout is not torch.strided:
+        raise ValueError(f"table must be a dense float32, bfloat16 or float16 tensor [K, ...] (got {kind} {tuple(shape)})")
+    if not isinstance(ids, torch.Tensor) or ids.device != device or ids.dtype not in _ID_TYPES:
         raise ValueError(f"ids must be an int32 or int64 tensor on {device}")
-    if ids.numel() >= 1 << 30 or table.shape[0] >= (1 << 31) - 1:
-        raise ValueError("at most 2^30 - 1 ids and 2^31 - 2 rows")
+    width = math.prod(shape[1:])
+    if ids.numel() >= 1 << 30 or shape[0] >= (1 << 31) - 1 or width > 1 << 22:
+        raise ValueError("at most 2^30 - 1 ids, 2^31 - 2 rows and 2^22 values in a row")
+    wanted = table.requires_grad
     if scale is None:
         scale = 1.0
-    if isinstance(scale, torch.Tensor):
+    elif isinstance(scale, torch.Tensor):
         if scale.device != device or scale.dtype != torch.float32 or scale.shape != ids.shape:
             raise ValueError(f"a scale tensor must be float32 {tuple(ids.shape)} on {device}, shaped like ids "
                              f"(got {scale.dtype} {tuple(scale.shape)} on {scale.device})")
+        wanted = wanted or scale.requires_grad
     else:
         scale = float(scale)
     if dtype is None:
-        dtype = table.dtype
-    elif dtype != table.dtype and dtype != torch.float32:
-        raise ValueError(f"the result has the table's type or float32 (got {dtype} for a table of {table.dtype})")
-    width = math.prod(table.shape[1:])
-    if width > 1 << 24:
-        raise ValueError("rows of more than 2^24 values")
-    if torch.is_grad_enabled() and (table.requires_grad or (isinstance(scale, torch.Tensor) and scale.requires_grad)):
+        dtype = kind
+    elif dtype != kind and dtype != torch.float32:
+        raise ValueError(f"the result has the table's type or float32 (got {dtype} for a table of {kind})")
+    if wanted and torch.is_grad_enabled():
         return _Lookup.apply(table, ids, scale, width, dtype)
     arguments, *keep = _arguments(table, ids, scale, width, dtype)
-    return _forward(arguments, ids.shape + table.shape[1:], dtype, device)
+    return _forward(arguments, ids.shape + shape[1:], dtype, device)
