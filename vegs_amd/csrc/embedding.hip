@@ -509,8 +509,28 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 
 // Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at JOIN_CHUNKS chunks; short
 // rows are one group's each, rows of more than JOIN_LONG pieces the whole workgroup's: group k adds the pieces k, k + groups, ... and
-// the groups' sums are added in order.
+// the groups' sums are added pairwise.
 constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 16, JOIN_AHEAD = 8;
+
+// The sums of a workgroup's groups, pairwise: group 0's lanes hold the result.  part: V floats for every thread, free before.
+template <int V>
+__device__ __forceinline__ void add_groups(float (&acc)[V], float* part, int g_shift)
+{
+    const int group = threadIdx.x >> g_shift;
+#pragma unroll
+    for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
+    __syncthreads();
+    for (int w = (int)(blockDim.x >> g_shift) >> 1; w > 0; w >>= 1) {
+        if (group < w) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                acc[v] += part[(threadIdx.x + (w << g_shift)) * V + v];
+                part[threadIdx.x * V + v] = acc[v];
+            }
+        }
+        __syncthreads();
+    }
+}
 
 // acc += the pieces p, p + step, ... up to `end` of the row whose tail is piece c, JOIN_AHEAD of them in flight
 template <int V>
@@ -557,11 +577,23 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         if (owner) {
             const int at = __popcll(mask & ((1ull << threadIdx.x) - 1ull));
             from[at] = c; row[at] = k;
+            // the last chunk whose first entry is of the row: one of the next four, or (-1) further on
+            int more = 0;
+            bool on = true;
+#pragma unroll
+            for (int x = 1; x <= 4; ++x) {
+                const long p = c + 1 + x < chunks ? c + 1 + x : c;
+                const bool same = q.key[p * q.chunk] == k && p != c;
+                on = on && same;
+                more += on;
+            }
+            upto[at] = more < 4 ? c + 1 + more : -1;
         }
     }
     __syncthreads();
-    // the last chunk whose first entry is of the row, a wave per row: chunks 1, 2, 4, ... further on at once, then 64 in between
+    // longer rows, a wave per row: chunks 1, 2, 4, ... further on at once, then 64 in between
     for (int o = threadIdx.x >> 6; o < count; o += JOIN_THREADS / 64) {
+        if (upto[o] >= 0) continue;
         const long base = from[o] + 1;
         const uint32_t k = row[o];
         const int at = threadIdx.x & 63;
@@ -601,21 +633,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
         join_pieces<V>(acc, slots, a.width, c, c + group, end, groups);
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
-        __syncthreads();
-        if (group == 0 && live) {
-            for (int k = 1; k < groups; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[v] += part[((k << q.g_shift) + lane) * V + v];
-            store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
-        }
+        add_groups<V>(acc, part, q.g_shift);
+        if (group == 0 && live) store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
     }
 }
 
 // ---- up to SMALL entries in one launch without any scratch: every workgroup sorts all of them in its LDS and writes the rows of its own
 // range, the ones without entries as zeros.  A row is one group's; one of more than SMALL_LONG entries is the whole workgroup's, in
-// contiguous pieces that are added in order.  (100 entries, 1000 rows of ten floats: 6 us against 12 for the three launches.)
+// contiguous pieces that are added pairwise.  (100 entries, 1000 rows of ten floats: 6 us against 12 for the three launches.)
 constexpr int SMALL = SORT_THREADS, SMALL_LONG = 32;
 
 __device__ __forceinline__ int first_at_least(const uint32_t* key, int n, uint32_t k)
@@ -717,15 +742,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_lookup_small(LookupArgs a, Sum
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
         if (from < upto) add_entries<TT, TO, V, DSCALE>(a, q, lds.val, from, upto, col, want, live, table + (long)k * a.table_stride, acc);
-#pragma unroll
-        for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
-        __syncthreads();
-        if (group == 0 && live) {
-            for (int g = 1; g < groups && g * each < end - j; ++g)
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[v] += part[((g << q.g_shift) + lane) * V + v];
-            store_row<TT, V>(d_table + (long)k * a.width, acc);
-        }
+        add_groups<V>(acc, part, q.g_shift);
+        if (group == 0 && live) store_row<TT, V>(d_table + (long)k * a.width, acc);
         __syncthreads();
     }
 }
@@ -769,11 +787,12 @@ static Tiling tiling(int64_t n, int64_t width, int v_full)
     t.g_shift = 0;
     while (t.g_shift < 6 && (1 << t.g_shift) < lanes) ++t.g_shift;
     t.tiles = (int)((lanes + 63) / 64);
-    // long chunks make few slots; shorter ones while there are fewer than four waves for each of the 1024 SIMDs -- but no more than
-    // 8192 of them, which is what one workgroup has to join where all entries are of one row (at 16384 entries of 1024 16-bit
-    // values: 13 us with four waves per SIMD, 19 with one)
+    // long chunks make few slots; shorter ones while there are fewer than four waves for each of the 1024 SIMDs (16384 entries of 1024
+    // 16-bit values: 13 us with four, 19 with one) -- but no more than 128 for each group of a join, which is what a row that all
+    // entries hit takes there one after the other
     t.chunk = 64;
-    while (t.chunk > UNROLL && ((n << t.g_shift) / 64 / t.chunk) * t.tiles < 4096 && n <= 4096l * t.chunk) t.chunk >>= 1;
+    const int64_t most = 128 * (JOIN_THREADS >> t.g_shift);
+    while (t.chunk > UNROLL && ((n << t.g_shift) / 64 / t.chunk) * t.tiles < 4096 && 2 * n <= most * t.chunk) t.chunk >>= 1;
     t.chunks = (long)((n + t.chunk - 1) / t.chunk);
     return t;
 }
