@@ -1,4 +1,12 @@
 // embedding.hip -- the row lookup and its gradients (include/vegs_embedding.h).
+//
+//   out[i] = s_i T[id_i]        dT[k] = sum_{i: id_i = k} s_i g_i        ds_i = <g_i, T[id_i]>
+//
+// Bound by memory: two operations per value.  Forward, the table is read from the caches and the result written once, streamed.
+// Backward, every gradient row is read once, in the order of the rows of T it goes to (a stable sort of the ids), so that a row's sum is
+// formed in registers without atomics, in an order that depends on the sizes alone.  Measured at 2 M entries of 45 floats, 8192
+// rows: forward 65 us (5.8 TB/s); sort 54, sums with the scales' gradient 150 (the rows of 180 bytes come as whole lines: 600 of their 360
+// MB), join 9.  Short inputs are bound by launches: up to 1024 entries take one, up to 16384 three.
 #include "../../include/vegs_embedding.h"
 #include "vr_host.h"
 #include "vr_types.h"
@@ -113,8 +121,16 @@ __global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict
 
 constexpr uint32_t NO_ENTRY = 0xffffffffu;            // behind every row and behind "no row"
 
-// ---- the sort of few entries by one workgroup: all of them stay in LDS through the passes (stable, 8 bits each).
-constexpr int SORT_SMALL = 16384, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+// between a wave's reads and writes of the same LDS words: the hardware keeps a wave's LDS operations in order, this the compiler's
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ---- the sort of few entries inside a workgroup: they stay in LDS through the passes (stable, digits of up to 8 bits).
+constexpr int SORT_SMALL = 16384, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_GROUPS = 16;
 
 template <int ITEMS>
 struct SortLds {
@@ -122,44 +138,50 @@ struct SortLds {
     uint32_t key[SORT_THREADS * ITEMS], val[SORT_THREADS * ITEMS];
 };
 
-// Entries 0 .. n - 1 by their row (`rows` for "no row", padding behind it) into lds.key / lds.val.  All SORT_THREADS threads; the
-// arrays may be read when it returns.
+// lds.key / lds.val [0, m), keys of `bits` bits from `lo` on, into ascending order.  All SORT_THREADS threads; the arrays have been
+// written and synchronised before, and may be read by everyone after.
 template <int ITEMS>
-__device__ __forceinline__ void sort_entries(const LookupArgs& a, int bits, SortLds<ITEMS>& lds)
+__device__ __forceinline__ void sort_in_lds(SortLds<ITEMS>& lds, int m, uint32_t lo, int bits)
 {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * ITEMS) + lane;
+    const int items = (m + SORT_THREADS - 1) / SORT_THREADS;                  // of each thread; what they are more than m stays last
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * items) + lane;
     const unsigned long long before = (1ull << lane) - 1ull;
     uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
-#pragma unroll
-    for (int x = 0; x < ITEMS; ++x) {
-        const int i = first + 64 * x;
-        const long row = i < a.n ? row_of(a, i) : -1;
-        key[x] = i < a.n ? (row >= 0 ? (uint32_t)row : (uint32_t)a.rows) : NO_ENTRY;
-        val[x] = (uint32_t)i;
-    }
     for (int shift = 0; shift < bits; shift += 8) {
+        const int digit_bits = bits - shift < 8 ? bits - shift : 8;
+        const uint32_t mask = (1u << digit_bits) - 1u;
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+            if (x < items) {
+                key[x] = lds.key[first + 64 * x];
+                val[x] = lds.val[first + 64 * x];
+            }
+        }
         for (int d = threadIdx.x; d < SORT_WAVES * 256; d += SORT_THREADS) (&lds.cnt[0][0])[d] = 0;
         __syncthreads();
         // the entry's place among those of its digit in its wave: lanes of the same digit by ballots, earlier items from the count
 #pragma unroll
         for (int x = 0; x < ITEMS; ++x) {
-            const uint32_t d = (key[x] >> shift) & 255u;
+            if (x >= items) continue;
+            const uint32_t d = first + 64 * x < m ? ((key[x] - lo) >> shift) & mask : mask;
             unsigned long long same = ~0ull;
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
+                if (b >= digit_bits) continue;
                 const unsigned long long on = __ballot((d >> b) & 1u);
                 same &= ((d >> b) & 1u) ? on : ~on;
             }
             const uint32_t prior = lds.cnt[w][d];
             rank[x] = prior + (uint32_t)__popcll(same & before);
-            __builtin_amdgcn_wave_barrier();
+            wave_order();
             if ((same & before) == 0) lds.cnt[w][d] = prior + (uint32_t)__popcll(same);
-            __builtin_amdgcn_wave_barrier();
+            wave_order();
         }
         __syncthreads();
         // exclusive sums over (digit, wave)
         uint32_t total = 0, incl = 0;
         if (threadIdx.x < 256) {
+#pragma unroll
             for (int k = 0; k < SORT_WAVES; ++k) {
                 const uint32_t c = lds.cnt[k][threadIdx.x];
                 lds.cnt[k][threadIdx.x] = total;
@@ -182,41 +204,87 @@ __device__ __forceinline__ void sort_entries(const LookupArgs& a, int bits, Sort
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < ITEMS; ++x) {
-            const uint32_t d = (key[x] >> shift) & 255u, at = lds.base[d] + lds.cnt[w][d] + rank[x];
+            if (x >= items) continue;
+            const uint32_t d = first + 64 * x < m ? ((key[x] - lo) >> shift) & mask : mask, at = lds.base[d] + lds.cnt[w][d] + rank[x];
             lds.key[at] = key[x];
             lds.val[at] = val[x];
         }
         __syncthreads();
-#pragma unroll
-        for (int x = 0; x < ITEMS; ++x) {
-            key[x] = lds.key[first + 64 * x];
-            val[x] = lds.val[first + 64 * x];
-        }
     }
 }
 
-// First launch for up to SORT_SMALL entries: one workgroup sorts, the others clear the gradient meanwhile.  (The general sort takes a
-// launch for the keys and four a pass: at 16384 entries and 32000 rows 49 us of kernels, and as much again between them; this one 35.)
-template <int ITEMS>
-__global__ void __launch_bounds__(SORT_THREADS)
-k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict__ val_out, int bits, char* __restrict__ zero, long zero_bytes)
+__device__ __forceinline__ uint32_t key_of(const LookupArgs& a, long i)
 {
+    const long row = row_of(a, i);
+    return row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
+}
+
+// First launch for up to SORT_SMALL entries.  SORT_GROUPS workgroups read all ids, take the entries of their own range of rows in order
+// into LDS, sort them there and write them behind the entries of smaller rows, which they have counted; the workgroups behind them clear
+// the gradient meanwhile.  (16384 entries of 32000 rows and 65 MB to clear: 40 us with one workgroup sorting all -- which is what it comes
+// to where all are of one range --, 24 with these; the general sort below takes six launches of 30 us together.)
+__global__ void __launch_bounds__(SORT_THREADS)
+k_lookup_sort(LookupArgs a, uint32_t* __restrict__ key_out, uint32_t* __restrict__ val_out, uint32_t range, int bits, char* __restrict__ zero,
+              long zero_bytes)
+{
+    constexpr int ITEMS = SORT_SMALL / SORT_THREADS;
     __shared__ SortLds<ITEMS> lds;
-    if (blockIdx.x > 0) {
-        zero_fill(zero, zero_bytes, (long)(blockIdx.x - 1) * SORT_THREADS + threadIdx.x, (long)(gridDim.x - 1) * SORT_THREADS);
+    __shared__ int in_range[SORT_WAVES], below[SORT_WAVES];
+    if (blockIdx.x >= SORT_GROUPS) {
+        zero_fill(zero, zero_bytes, (long)(blockIdx.x - SORT_GROUPS) * SORT_THREADS + threadIdx.x,
+                  (long)(gridDim.x - SORT_GROUPS) * SORT_THREADS);
         return;
     }
-    sort_entries<ITEMS>(a, bits, lds);
-    for (int i = threadIdx.x; i < a.n; i += SORT_THREADS) {
-        key_out[i] = lds.key[i];
-        val_out[i] = lds.val[i];
+    const int n = (int)a.n, items = (n + SORT_THREADS - 1) / SORT_THREADS;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, first = w * (64 * items) + lane;
+    const unsigned long long before = (1ull << lane) - 1ull;
+    const uint32_t lo = blockIdx.x * range;                        // (the last range holds "no row" too, or lies behind it)
+    int mine = 0, smaller = 0;
+    uint32_t key[ITEMS];
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        if (x >= items) continue;
+        const int i = first + 64 * x;
+        key[x] = i < n ? key_of(a, i) : NO_ENTRY;
+    }
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        if (x >= items) continue;
+        mine += __popcll(__ballot(key[x] >= lo && key[x] - lo < range && key[x] != NO_ENTRY));
+        smaller += __popcll(__ballot(key[x] < lo));
+    }
+    if (lane == 0) { in_range[w] = mine; below[w] = smaller; }
+    __syncthreads();
+    int at = 0, m = 0, out = 0;
+    for (int k = 0; k < SORT_WAVES; ++k) {
+        at += k < w ? in_range[k] : 0;
+        m += in_range[k];
+        out += below[k];
+    }
+#pragma unroll
+    for (int x = 0; x < ITEMS; ++x) {
+        if (x >= items) continue;
+        const bool in = key[x] >= lo && key[x] - lo < range && key[x] != NO_ENTRY;
+        const unsigned long long on = __ballot(in);
+        if (in) {
+            const int to = at + __popcll(on & before);
+            lds.key[to] = key[x];
+            lds.val[to] = (uint32_t)(first + 64 * x);
+        }
+        at += __popcll(on);
+    }
+    __syncthreads();
+    sort_in_lds<ITEMS>(lds, m, lo, bits);
+    for (int i = threadIdx.x; i < m; i += SORT_THREADS) {
+        key_out[out + i] = lds.key[i];
+        val_out[out + i] = lds.val[i];
     }
 }
 
 // ---- the sort of many entries: stable, least significant digit first, digits of up to 8 bits; a pass is a histogram per block of
 // SORT_BLOCK entries, the sums over the blocks of each digit, and the scatter.  The first pass takes its keys from the ids, and its
 // histogram's launch clears the table's gradient in further workgroups.  The scales travel with the entries: gathered afterwards, every
-// one of them would fetch a line of its own (2 M entries: 23 us of the sums' 162, 5 us here).
+// one of them would fetch a line of its own (2 M entries: the sums 7 us longer, the passes 1 each shorter).
 constexpr int SORT_BLOCK = 4096, PASS_THREADS = 1024, PASS_WAVES = PASS_THREADS / 64, PASS_ITEMS = SORT_BLOCK / PASS_THREADS;
 
 struct PassArgs {
@@ -231,8 +299,7 @@ struct PassArgs {
 __device__ __forceinline__ uint32_t pass_key(const LookupArgs& a, const PassArgs& p, long i)
 {
     if (p.key) return p.key[i];
-    const long row = row_of(a, i);
-    return row >= 0 ? (uint32_t)row : (uint32_t)a.rows;
+    return key_of(a, i);
 }
 
 __global__ void __launch_bounds__(PASS_THREADS) k_sort_hist(LookupArgs a, PassArgs p, char* __restrict__ zero, long zero_bytes)
@@ -321,9 +388,9 @@ __global__ void __launch_bounds__(PASS_THREADS) k_sort_scatter(LookupArgs a, Pas
         }
         const uint32_t prior = cnt[w][d];
         rank[x] = prior + (uint32_t)__popcll(same & before);
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
         if (in && (same & before) == 0) cnt[w][d] = prior + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
     }
     __syncthreads();
     // per digit: where the waves' entries begin in the block, and where the block's begin among all
@@ -467,6 +534,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
                     acc[v] = fmaf(sx, gv, acc[v]);
                     if (DSCALE && col + v >= want) dot[x] = fmaf(gv, load_f32(t_cur.v + v), dot[x]);
                 }
+                if (DSCALE) dot[x] *= a.scale;
             }
         }
         if (DSCALE) {
@@ -489,12 +557,12 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
                 }
                 for (; w > 0; w >>= 1) d[0] += __shfl_xor(d[0], w, 64);
                 const int x = lane >> (q.g_shift - U_SHIFT);
-                if ((lane & ((G >> U_SHIFT) - 1)) == 0 && j + x < last) q.d_row_scale[q.val[j + x]] = a.scale * d[0];
+                if ((lane & ((G >> U_SHIFT) - 1)) == 0 && j + x < last) q.d_row_scale[q.val[j + x]] = d[0];
             } else {
 #pragma unroll
                 for (int x = 0; x < U; ++x) {
                     for (int w = G >> 1; w > 0; w >>= 1) d[x] += __shfl_xor(d[x], w, 64);
-                    if (lane == 0 && j + x < last) q.d_row_scale[val[x]] = a.scale * d[x];
+                    if (lane == 0 && j + x < last) q.d_row_scale[val[x]] = d[x];
                 }
             }
         }
@@ -640,7 +708,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
 
 // ---- up to SMALL entries in one launch without any scratch: every workgroup sorts all of them in its LDS and writes the rows of its own
 // range, the ones without entries as zeros.  A row is one group's; one of more than SMALL_LONG entries is the whole workgroup's, in
-// contiguous pieces that are added pairwise.  (100 entries, 1000 rows of ten floats: 6 us against 12 for the three launches.)
+// contiguous pieces that are added pairwise.  (100 entries, 1000 rows of ten floats: 9 us against 12 in three launches.)
 constexpr int SMALL = SORT_THREADS, SMALL_LONG = 32;
 
 __device__ __forceinline__ int first_at_least(const uint32_t* key, int n, uint32_t k)
@@ -696,9 +764,15 @@ __global__ void __launch_bounds__(SORT_THREADS) k_lookup_small(LookupArgs a, Sum
     __shared__ SortLds<1> lds;
     __shared__ float part[SORT_THREADS * V];
     __shared__ int long_runs[SMALL / SMALL_LONG], n_long;
+    const int n = (int)a.n;
     if (threadIdx.x == 0) n_long = 0;
-    sort_entries<1>(a, bits, lds);
-    const int n = (int)a.n, G = 1 << q.g_shift, lane = threadIdx.x & (G - 1), group = threadIdx.x >> q.g_shift, groups = SORT_THREADS >> q.g_shift;
+    if ((int)threadIdx.x < n) {
+        lds.key[threadIdx.x] = key_of(a, threadIdx.x);
+        lds.val[threadIdx.x] = threadIdx.x;
+    }
+    __syncthreads();
+    sort_in_lds<1>(lds, n, 0, bits);
+    const int G = 1 << q.g_shift, lane = threadIdx.x & (G - 1), group = threadIdx.x >> q.g_shift, groups = SORT_THREADS >> q.g_shift;
     const long r0 = (long)blockIdx.x * rows_each, r1 = r0 + rows_each < a.rows ? r0 + rows_each : a.rows;
     const long want = ((long)blockIdx.y * G + lane) * V;
     const bool live = want < a.width;
@@ -771,7 +845,7 @@ __global__ void __launch_bounds__(256) k_lookup_dscale(LookupArgs a, const TO* _
         }
     }
     for (int w = G >> 1; w > 0; w >>= 1) acc += __shfl_xor(acc, w, 64);
-    if (lane == 0) d_row_scale[i] = a.scale * acc;
+    if (lane == 0) d_row_scale[i] = row >= 0 ? a.scale * acc : 0.0f;
 }
 
 // Lanes and columns for a width: V values (16 bytes of the result's type) per lane, or one where the row is shorter than that.
@@ -953,11 +1027,10 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
         const long zero_bytes = a.rows * a.width * (long)t_element, zero_blocks = (zero_bytes + 16383) / 16384;
         const int bits = key_bits(a.rows);
         if (a.n <= SORT_SMALL) {
-            const dim3 grid(1 + (unsigned)(zero_blocks < 1024 ? zero_blocks : 1024));
-            if (a.n <= 4 * SORT_THREADS)
-                hipLaunchKernelGGL(k_lookup_sort<4>, grid, dim3(SORT_THREADS), 0, s, a, key[0], val[0], bits, (char*)d_table, zero_bytes);
-            else
-                hipLaunchKernelGGL(k_lookup_sort<16>, grid, dim3(SORT_THREADS), 0, s, a, key[0], val[0], bits, (char*)d_table, zero_bytes);
+            const dim3 grid(SORT_GROUPS + (unsigned)(zero_blocks < 1024 ? zero_blocks : 1024));
+            const uint32_t range = (uint32_t)((a.rows + SORT_GROUPS) / SORT_GROUPS);          // of the keys 0 .. rows
+            hipLaunchKernelGGL(k_lookup_sort, grid, dim3(SORT_THREADS), 0, s, a, key[0], val[0], range, key_bits((int64_t)range - 1),
+                               (char*)d_table, zero_bytes);
             VR_KERNEL_CHECK("lookup_sort", s, false);
             q.key = key[0];
             q.val = val[0];
