@@ -2,11 +2,11 @@
 //
 //   norm = sqrt(sum over all tensors of g^2)   or   max |g|;      g *= min(1, max_norm / (norm + 1e-6))
 //
-// Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more, and only when the factor is
-// not one.  The squares are taken and added in fp64: a product of two fp32 values is exact there and neither overflows
-// nor vanishes, and the vector ALUs do 64-bit multiply-adds an order of magnitude faster than memory delivers operands.
-// No atomics: every workgroup writes one partial result and one last workgroup adds them in a fixed order, so that the ranks of a
-// job that hold the same gradients clip by the same bits.
+// Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more, and only when the factor is not
+// one (118 M fp32 elements: 80 us, 5.9 TB/s, and 149 us, 6.3 TB/s).  The squares are taken and added in fp64: a product of two
+// fp32 values is exact there and neither overflows nor vanishes, and the vector ALUs do 64-bit multiply-adds an order of
+// magnitude faster than memory delivers operands.  No atomics: every workgroup writes one partial result, and they are added in
+// one fixed order, so that the ranks of a job that hold the same gradients clip by the same bits.
 #include "../../include/vegs_optim.h"
 #include "vr_host.h"
 #include "vr_sh_factors.h"
@@ -166,7 +166,6 @@ __device__ __forceinline__ void scale_unit(void* data, long base, long n, float 
     }
 }
 
-// From the last unit to the first: the norm's pass ended there, and what it read last is still in the memory-side cache.
 // The norm comes from memory, or (KIND 1: sum of squares, 2: largest magnitude) from k_grad_norm's partial results, which every workgroup
 // adds up for itself -- at most 16 KB from the L2 each, and a launch less between the two passes.
 template <int KIND, int LOADS>
@@ -188,8 +187,7 @@ __global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, float* __restric
         c = clip_factor(*norm, max_norm);
     }
     if (c == 1.0f) return;
-    for (int k = blockIdx.x; k < a.units; k += gridDim.x) {
-        const int unit = a.units - 1 - k;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const GradSeg s = grad_seg(a, unit);
         const long at = (long)(unit - s.unit0) * (LOADS * GN_LOAD_BYTES);
         if (s.dtype == VR_F32) scale_unit<float, LOADS>(s.data, at / 4, s.n, c);

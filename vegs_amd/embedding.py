@@ -58,30 +58,41 @@ def _forward(arguments, shape, dtype, device):
             return _forward(arguments, shape, dtype, device)
     out = torch.empty(shape, dtype=dtype, device=device)
     if out.numel():
-        _capi.check(_capi.load().vr_lookup_forward(arguments, out.data_ptr(), _capi.stream_of(device)))
+        rc = (_capi._lib or _capi.load()).vr_lookup_forward(arguments, out.data_ptr(), _capi.stream_of(device))
+        if rc:
+            _capi.check(rc)
     return out
 
 
 def _backward(ctx, g):
-    keep = ctx.saved_tensors                      # (what ctx.arguments points at, as far as it is read)
-    arguments, shape, dtype, n, width = ctx.arguments, ctx.shape, ctx.dtype, ctx.n, ctx.width
+    keep = ctx.saved_tensors                      # (what the arguments point at, as far as it is read)
+    device, index = g.device, g.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _backward(ctx, g)
+    arguments, shape, dtype, ids_shape, n, width = ctx.lookup
     want_table, _, want_scale, _, _ = ctx.needs_input_grad
-    device = g.device
-    with _capi.on(device):
-        d_table = torch.empty(shape, dtype=dtype, device=device) if want_table else None
-        d_scale = torch.empty(ctx.ids_shape, dtype=torch.float32, device=device) if want_scale else None
-        if width == 0 or n == 0:
-            return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
-        stride = width
-        if not g.is_contiguous():
-            g, stride = _row_layout(g, len(ctx.ids_shape), width)
-        lib = _capi.load()
-        scratch = None
-        nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width) if want_table else 0
-        if nbytes:
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _capi.check(lib.vr_lookup_backward(arguments, g.data_ptr(), stride, _capi.ptr(d_table), _capi.ptr(d_scale),
-                                           _capi.ptr(scratch), nbytes, _capi.stream_of(device)))
+    d_table = d_scale = scratch = None
+    nbytes = at_table = at_scale = 0
+    lib = _capi._lib or _capi.load()
+    if want_table:
+        d_table = torch.empty(shape, dtype=dtype, device=device)
+        at_table = d_table.data_ptr()
+        nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width)
+    if want_scale:
+        d_scale = torch.empty(ids_shape, dtype=torch.float32, device=device)
+        at_scale = d_scale.data_ptr()
+    if width == 0 or n == 0:
+        return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
+    stride = width
+    if not g.is_contiguous():
+        g, stride = _row_layout(g, len(ids_shape), width)
+    if nbytes:
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    rc = lib.vr_lookup_backward(arguments, g.data_ptr(), stride, at_table, at_scale, scratch.data_ptr() if nbytes else None, nbytes,
+                                _capi.stream_of(device))
+    if rc:
+        _capi.check(rc)
     return d_table, None, d_scale, None, None
 
 
@@ -92,11 +103,11 @@ class _Lookup(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, ids, scale, width, dtype):
-        ctx.arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
-        ctx.shape, ctx.dtype, ctx.ids_shape, ctx.n, ctx.width = table.shape, table.dtype, ids.shape, ids.numel(), width
+        arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
+        ctx.lookup = arguments, table.shape, table.dtype, ids.shape, ids.numel(), width
         # (the table's values are only read again for the gradient of the scales)
         ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, flat, scales)
-        return _forward(ctx.arguments, ids.shape + table.shape[1:], dtype, table.device)
+        return _forward(arguments, ids.shape + table.shape[1:], dtype, table.device)
 
     @staticmethod
     def backward(ctx, g):
