@@ -5,8 +5,8 @@
 // Bound by memory: two operations per value.  Forward, the table is read from the caches and the result written once, streamed.
 // Backward, every gradient row is read once, in the order of the rows of T it goes to (a stable sort of the ids), so that a row's sum is
 // formed in registers without atomics, in an order that depends on the sizes alone.  Measured at 2 M entries of 45 floats, 8192
-// rows: forward 65 us (5.8 TB/s); sort 54, sums with the scales' gradient 150 (the rows of 180 bytes come as whole lines: 600 of their 360
-// MB), join 9.  Short inputs are bound by launches: up to 1024 entries take one, up to 16384 three.
+// rows: forward 65 us (5.8 TB/s); sort 53, sums with the scales' gradient 141 (the rows of 180 bytes come as whole lines: 600 MB for their
+// 360), join 12.  Short inputs are bound by launches: up to 1024 entries take one, up to 16384 three.
 #include "../../include/vegs_embedding.h"
 #include "vr_host.h"
 #include "vr_types.h"
@@ -501,15 +501,12 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
             val[x] = in ? (&v4[x / 4].x)[x % 4] : 0u;
         }
         Pack<TO, V> g[U];
-        Pack<TT, V> t[U];
         float s[U];
 #pragma unroll
         for (int x = 0; x < U; ++x) {
             const bool there = key[x] < rows;
             s[x] = q.scales ? q.scales[j + x] : there && a.row_scale ? a.row_scale[val[x]] : 1.0f;     // (padded as the keys)
             g[x] = load_once<TO, V>(grad + (there ? (long)val[x] * q.grad_stride : 0));
-            // (a row of the table is read where it begins among the entries, not again for each of them)
-            if (DSCALE && there && key[x] != (x == 0 ? cur : key[x - 1])) t[x] = *reinterpret_cast<const Pack<TT, V>*>(table + (long)key[x] * a.table_stride);
         }
         float dot[U];
 #pragma unroll
@@ -521,7 +518,10 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
                 }
                 came_in = false;
                 cur = key[x];
-                if (DSCALE) t_cur = t[x];
+                // (the row of the table is waited for here: reading all that begin among the U ahead of time takes registers for
+                // eight of them and with those a wave per SIMD -- 152 us against 141 at 244 entries a row, 192 against 195 at 4,
+                // 282 against 297 at one)
+                if (DSCALE && cur < rows) t_cur = *reinterpret_cast<const Pack<TT, V>*>(table + (long)cur * a.table_stride);
 #pragma unroll
                 for (int v = 0; v < V; ++v) acc[v] = 0.0f;
             }
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
         if (DSCALE) {
             // the group's sums of the U products.  Where it has as many lanes, half of them pass on the half of the sums
             // that the others keep, three times, so that every eighth of the lanes ends with one sum: 8 exchanges and one store
-            // for 16 lanes where a butterfly for each sum takes 32 and eight (2 M x 45: 150 us against 155)
+            // for 16 lanes where a butterfly for each sum takes 32 and eight (2 M x 45: 3 % of the kernel)
             float d[U];
 #pragma unroll
             for (int x = 0; x < U; ++x) d[x] = live ? dot[x] : 0.0f;
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
     }
 }
 
-// Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at JOIN_CHUNKS chunks; short
+// Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at up to JOIN_CHUNKS chunks; short
 // rows are one group's each, rows of more than JOIN_LONG pieces the whole workgroup's: group k adds the pieces k, k + groups, ... and
 // the groups' sums are added pairwise.
 constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 16, JOIN_AHEAD = 8;
@@ -621,7 +621,7 @@ __device__ __forceinline__ void join_pieces(float (&acc)[V], const float* __rest
 }
 
 template <typename TT, int V>
-__global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumArgs q, long chunks)
+__global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumArgs q, long chunks, int each)
 {
     __shared__ long from[JOIN_CHUNKS], upto[JOIN_CHUNKS];
     __shared__ uint32_t row[JOIN_CHUNKS];
@@ -632,10 +632,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
     const bool live = want < a.width;
     const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
     if (threadIdx.x < JOIN_CHUNKS) {
-        const long c = (long)blockIdx.x * JOIN_CHUNKS + threadIdx.x, first = c * q.chunk, next = first + q.chunk;
+        const long c = (long)blockIdx.x * each + threadIdx.x, first = c * q.chunk, next = first + q.chunk;
         bool owner = false;
         uint32_t k = 0;
-        if (c < chunks && next < a.n) {
+        if ((int)threadIdx.x < each && c < chunks && next < a.n) {
             k = q.key[next - 1];
             // its last row goes on, and begins in this chunk
             owner = k < (uint32_t)a.rows && q.key[next] == k && (first == 0 || q.key[first - 1] != k);
@@ -937,9 +937,11 @@ struct Backward {
             const dim3 grid((unsigned)(((t.chunks << t.g_shift) + 255) / 256), t.tiles);
             if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, true>), grid, dim3(256), 0, s, a, q);
             else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, false>), grid, dim3(256), 0, s, a, q);
+            // (few chunks: fewer a workgroup, so that each of its groups has one row at most)
+            const int each = t.chunks > 8192 ? JOIN_CHUNKS : JOIN_CHUNKS / 4;
             if (t.chunks > 1)
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_join<TT, V>), dim3((unsigned)((t.chunks + JOIN_CHUNKS - 1) / JOIN_CHUNKS), t.tiles),
-                                   dim3(JOIN_THREADS), 0, s, a, q, t.chunks);
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_join<TT, V>), dim3((unsigned)((t.chunks + each - 1) / each), t.tiles),
+                                   dim3(JOIN_THREADS), 0, s, a, q, t.chunks, each);
         }
         if (q.d_row_scale && !fused)
             hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_dscale<TT, TO, V>), dim3((unsigned)(((a.n << t.g_shift) + 255) / 256)), dim3(256),
