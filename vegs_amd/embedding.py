@@ -5,8 +5,9 @@
 
 What a model shares between its Gaussians, frames or instances is held once and looked up: an SH codebook (table [K, 15, 3],
 one id per Gaussian; the result IS the f_rest input of the rasterizer, next to instances.activate's outputs), per-image codes,
-pose corrections by frame.  The table's gradient is dense, in the table's type, so vegs_amd.optim.Adam, grad_norm and the
-exchanges of vegs_amd.dist take it like any other.  GPU tensors only; there is no CPU path.
+pose corrections by frame.  The table's gradient is dense, in the table's type: a float32 table is stepped by
+vegs_amd.optim.Adam, counted by grad_norm and exchanged by vegs_amd.dist like any other parameter.  GPU tensors only; there
+is no CPU path.
 """
 import math
 import struct
@@ -123,7 +124,7 @@ def lookup(table, ids, scale=None, dtype=None):
     tensor shaped like ids.  dtype: of the result, the table's (default) or float32.
 
     The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in float32, in an order
-    that the sizes fix, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same
+    that the sizes and ids fix, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same
     bits every time."""
     if not isinstance(table, torch.Tensor) or not table.is_cuda:
         raise ValueError("table must be a GPU tensor (there is no CPU path)")
