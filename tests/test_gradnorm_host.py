@@ -97,3 +97,12 @@ def test_gradients_that_fill_their_memory_are_told_from_others():
     assert optim._dense(t) and optim._dense(t.permute(2, 0, 1)) and optim._dense(t[1]) and optim._dense(t[:, :1].squeeze(1)[:0])
     assert not optim._dense(t[:, ::2]) and not optim._dense(t[:, :, 1:]) and not optim._dense(torch.zeros(1).expand(7))
     assert optim._dense(t[:, :1, :1][:1])                # one element: its strides say nothing
+
+
+def test_sparse_gradients_are_refused():
+    p = torch.nn.Parameter(torch.zeros(4, 3))
+    p.grad = torch.sparse_coo_tensor([[1]], [[1.0, 2.0, 3.0]], (4, 3))
+    with pytest.raises(ValueError, match="dense"):
+        optim.grad_norm([p])
+    with pytest.raises(ValueError, match="dense"):
+        optim.clip_grad_norm_([p], 1.0)
