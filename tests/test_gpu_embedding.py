@@ -112,6 +112,31 @@ def test_types(dtype, out, width, scale, index):
     _check(table, ids, scale, g, out)
 
 
+# more entries than one workgroup sorts alone (1024), and more than sixteen sort by ranges of rows (16384): sums in chunks
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 31, 33, 45, 48, 64, 65, 128, 129, 255, 257, 512, 513, 1025, 2051])
+@pytest.mark.parametrize("n,kind", [(1500, "holes"), (5000, "hot"), (17000, "holes"), (17000, "ends")])
+def test_widths_in_chunks(width, n, kind):
+    _check(*_inputs(n, 300, width, kind, seed=width, whole=True), exact=True)
+    _check(*_inputs(n, 300, width, kind, BF16, seed=width + 1))
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("width", [3, 8, 45, 600])
+@pytest.mark.parametrize("scale", ["row", None, -1.75])
+@pytest.mark.parametrize("n", [3000, 20000])
+def test_types_in_chunks(dtype, out, width, scale, n):
+    for index in (torch.int32, torch.int64):
+        table, ids, scale_, g = _inputs(n, 700, width, "holes", dtype, out, scale, index, seed=3)
+        _check(table, ids, scale_, g, out)
+
+
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 255, 256, 4095, 4096, 70000])
+@pytest.mark.parametrize("n", [1025, 16384, 16385])
+@pytest.mark.parametrize("kind", ["uniform", "same", "holes"])
+def test_rows_at_the_borders_of_the_sorts(rows, n, kind):
+    _check(*_inputs(n, rows, 6, kind, seed=rows, whole=True), exact=True)
+
+
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 31, 32, 33, 63, 64, 65, 255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096,
                                4097, 8193, 20011])
 @pytest.mark.parametrize("kind", ["uniform", "same", "hot", "runs", "ends", "holes", "none"])
@@ -307,7 +332,7 @@ def test_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(got[k], want[k % 4]))
 
 
-@pytest.mark.parametrize("n", [100, 30000])
+@pytest.mark.parametrize("n", [100, 5000, 30000])
 def test_captured_and_replayed(n):
     """A training step's lookup and gradients in a graph, twice, replayed with other inputs and eager work between."""
     from vegs_amd import embedding
