@@ -3,7 +3,7 @@
 //   norm = sqrt(sum over all tensors of g^2)   or   max |g|;      g *= min(1, max_norm / (norm + 1e-6))
 //
 // Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more, and only when the factor is not
-// one (118 M fp32 elements: 80 us, 5.9 TB/s, and 149 us, 6.3 TB/s).  The squares are taken and added in fp64: a product of two
+// one (118 M fp32 elements: 76 us, 6.2 TB/s, and 152 us, 6.2 TB/s).  The squares are taken and added in fp64: a product of two
 // fp32 values is exact there and neither overflows nor vanishes, and the vector ALUs do 64-bit multiply-adds an order of
 // magnitude faster than memory delivers operands.  No atomics: every workgroup writes one partial result, and they are added in
 // one fixed order, so that the ranks of a job that hold the same gradients clip by the same bits.
@@ -15,9 +15,10 @@
 namespace vr {
 
 constexpr int GN_MAX_T = 128;              // tensors per launch: the table is a kernel argument, 128 x 24 B of its 4 KB
-constexpr int GN_LOADS = 4;                // 16-byte loads a thread has in flight, so a workgroup's unit is 16 KB; 4 KB units
-constexpr int GN_LOAD_BYTES = 256 * 16;    // (one load) where that would leave CUs without work
-constexpr int GN_GRID = 2048;              // workgroups of a launch at most: eight for each of the 256 CUs
+// A thread has two 16-byte loads in flight, a workgroup's unit is 8 KB, and 1024 workgroups -- four for each of the 256 CUs -- go
+// through the units in turns.  (118 M fp32 elements: 76 us; with 2048 workgroups 81 for two, four and eight loads alike.  18 M bf16
+// elements, the largest magnitude: 11 us, 14 for four loads, 21 for eight, whose unpacked values wait on one another.)
+constexpr int GN_LOADS = 2, GN_UNIT = GN_LOADS * 256 * 16, GN_GRID = 1024;
 
 struct GradSeg {
     void* data;
@@ -27,7 +28,7 @@ struct GradSeg {
 };
 struct GradArgs {
     GradSeg seg[GN_MAX_T];
-    int count, units, loads;
+    int count, units;
 };
 
 // 16 bytes of values at an address of their own alignment (a gradient may be a view that starts anywhere)
@@ -76,20 +77,20 @@ __device__ __forceinline__ GradSeg grad_seg(const GradArgs& a, int unit)
     return a.seg[t];
 }
 
-// A unit's values: LOADS loads of 16 bytes per thread at once where the unit is full, single values in a tensor's last unit.
+// A unit's values: the thread's loads at once where the unit is full, single values in a tensor's last unit.
 // Two accumulators, for the 64-bit multiply-add's latency.
-template <typename T, int LOADS, typename A>
+template <typename T, typename A>
 __device__ __forceinline__ void norm_unit(const void* data, long base, long n, A& acc0, A& acc1)
 {
     constexpr int V = 16 / sizeof(T), PER = 256 * V;
     const T* p = reinterpret_cast<const T*>(data) + base;
     const long left = n - base;
-    if (left >= LOADS * PER) {
-        Quad<T> q[LOADS];
+    if (left >= GN_LOADS * PER) {
+        Quad<T> q[GN_LOADS];
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+        for (int j = 0; j < GN_LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
+        for (int j = 0; j < GN_LOADS; ++j)
 #pragma unroll
             for (int v = 0; v < V; v += 2) {
                 acc0 = norm_add(acc0, load_f32(q[j].v + v));
@@ -100,7 +101,7 @@ __device__ __forceinline__ void norm_unit(const void* data, long base, long n, A
     }
 }
 
-template <bool MAX, int LOADS>
+template <bool MAX>
 __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restrict__ partial)
 {
     using A = typename Acc<MAX>::type;
@@ -108,15 +109,16 @@ __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restric
     A acc = 0, acc1 = 0;
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const GradSeg s = grad_seg(a, unit);
-        const long at = (long)(unit - s.unit0) * (LOADS * GN_LOAD_BYTES);
-        if (s.dtype == VR_F32) norm_unit<float, LOADS>(s.data, at / 4, s.n, acc, acc1);
-        else if (s.dtype == VR_BF16) norm_unit<bf16, LOADS>(s.data, at / 2, s.n, acc, acc1);
-        else norm_unit<__half, LOADS>(s.data, at / 2, s.n, acc, acc1);
+        const long at = (long)(unit - s.unit0) * GN_UNIT;
+        if (s.dtype == VR_F32) norm_unit<float>(s.data, at / 4, s.n, acc, acc1);
+        else if (s.dtype == VR_BF16) norm_unit<bf16>(s.data, at / 2, s.n, acc, acc1);
+        else norm_unit<__half>(s.data, at / 2, s.n, acc, acc1);
     }
     acc = norm_block(norm_join(acc, acc1), lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
+// (2 M Gaussians, degree 3: 22 us for one view, 41 for four; the dense gradient would be 384 MB to write and read.)
 // One Gaussian per thread: its dense SH row is rebuilt in registers, from the same function the optimizer's kernel
 // steps with, and only its squares leave.
 template <bool MAX>
@@ -145,18 +147,18 @@ __global__ void __launch_bounds__(256) k_grad_norm_finish(const double* __restri
     if (threadIdx.x == 0) norm[0] = x;
 }
 
-template <typename T, int LOADS>
+template <typename T>
 __device__ __forceinline__ void scale_unit(void* data, long base, long n, float c)
 {
     constexpr int V = 16 / sizeof(T), PER = 256 * V;
     T* p = reinterpret_cast<T*>(data) + base;
     const long left = n - base;
-    if (left >= LOADS * PER) {
-        Quad<T> q[LOADS];
+    if (left >= GN_LOADS * PER) {
+        Quad<T> q[GN_LOADS];
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
+        for (int j = 0; j < GN_LOADS; ++j) q[j] = *reinterpret_cast<const Quad<T>*>(p + j * PER + threadIdx.x * V);
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
+        for (int j = 0; j < GN_LOADS; ++j) {
 #pragma unroll
             for (int v = 0; v < V; ++v) store_f32(q[j].v + v, c * load_f32(q[j].v + v));
             *reinterpret_cast<Quad<T>*>(p + j * PER + threadIdx.x * V) = q[j];
@@ -167,8 +169,8 @@ __device__ __forceinline__ void scale_unit(void* data, long base, long n, float 
 }
 
 // The norm comes from memory, or (KIND 1: sum of squares, 2: largest magnitude) from k_grad_norm's partial results, which every workgroup
-// adds up for itself -- at most 16 KB from the L2 each, and a launch less between the two passes.
-template <int KIND, int LOADS>
+// adds up for itself -- 8 KB a launch from the L2 each, and a launch less between the two passes.
+template <int KIND>
 __global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, float* __restrict__ norm, float max_norm,
                                                     const double* __restrict__ partial, int n_partial)
 {
@@ -189,10 +191,10 @@ __global__ void __launch_bounds__(256) k_clip_grads(GradArgs a, float* __restric
     if (c == 1.0f) return;
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         const GradSeg s = grad_seg(a, unit);
-        const long at = (long)(unit - s.unit0) * (LOADS * GN_LOAD_BYTES);
-        if (s.dtype == VR_F32) scale_unit<float, LOADS>(s.data, at / 4, s.n, c);
-        else if (s.dtype == VR_BF16) scale_unit<bf16, LOADS>(s.data, at / 2, s.n, c);
-        else scale_unit<__half, LOADS>(s.data, at / 2, s.n, c);
+        const long at = (long)(unit - s.unit0) * GN_UNIT;
+        if (s.dtype == VR_F32) scale_unit<float>(s.data, at / 4, s.n, c);
+        else if (s.dtype == VR_BF16) scale_unit<bf16>(s.data, at / 2, s.n, c);
+        else scale_unit<__half>(s.data, at / 2, s.n, c);
     }
 }
 
@@ -264,14 +266,9 @@ static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
 {
     int next = first;
     a.count = a.units = 0;
-    // one load a thread unless that fills the largest grid
-    int64_t bytes = 0;
-    for (int i = first; i < count && i < first + GN_MAX_T; ++i) bytes += t[i].n * (t[i].dtype == VR_F32 ? 4 : 2);
-    a.loads = bytes > (int64_t)GN_GRID * GN_LOAD_BYTES ? GN_LOADS : 1;
-    const long unit = (long)a.loads * GN_LOAD_BYTES;
     for (; next < count && a.count < GN_MAX_T; ++next) {
         if (t[next].n == 0) continue;
-        const long units = (t[next].n * (t[next].dtype == VR_F32 ? 4 : 2) + unit - 1) / unit;
+        const long units = (t[next].n * (t[next].dtype == VR_F32 ? 4 : 2) + GN_UNIT - 1) / GN_UNIT;
         if (a.units + units > 0x3fffffff) break;
         a.seg[a.count++] = GradSeg{t[next].data, (long)t[next].n, a.units, (int)t[next].dtype};
         a.units += (int)units;
@@ -283,9 +280,7 @@ static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
 template <int KIND>
 static void launch_clip(const GradArgs& a, float* norm, float max_norm, const double* partial, int n, hipStream_t s)
 {
-    const dim3 grid(a.units < GN_GRID ? a.units : GN_GRID);
-    if (a.loads == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_clip_grads<KIND, 1>), grid, dim3(256), 0, s, a, norm, max_norm, partial, n);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_clip_grads<KIND, GN_LOADS>), grid, dim3(256), 0, s, a, norm, max_norm, partial, n);
+    hipLaunchKernelGGL(k_clip_grads<KIND>, dim3(a.units < GN_GRID ? a.units : GN_GRID), dim3(256), 0, s, a, norm, max_norm, partial, n);
 }
 
 // clip: scale as well
@@ -307,8 +302,7 @@ static int grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradF
         first = fill_grads(tensors, first, count, a);
         if (a.units == 0) continue;
         const int grid = a.units < GN_GRID ? a.units : GN_GRID;
-        if (a.loads == 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm<MAX, 1>), dim3(grid), dim3(256), 0, s, a, partial + n);
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_grad_norm<MAX, GN_LOADS>), dim3(grid), dim3(256), 0, s, a, partial + n);
+        hipLaunchKernelGGL(k_grad_norm<MAX>, dim3(grid), dim3(256), 0, s, a, partial + n);
         n += grid;
     }
     for (int i = 0; i < n_factors; ++i) {
