@@ -330,8 +330,8 @@ __device__ __forceinline__ void bwd_chunk_trips(const int lane, const int e, con
         // The forward's own 2^x (bit for bit: same operations), not the hardware's: WHICH fragments contributed is
         // the forward's decision (alpha >= 1/255), and v_exp_f32 agrees with it only to ~2 ulp -- rare to matter,
         // but a faint splat has ALL its fragments at the threshold, and one fragment of twenty classified the other
-        // way moved its gradient by 4.5 % (the C-harness test caught it).  Evaluated for both pixels in packed
-        // arithmetic; +14 us per view over two v_exp_f32 -- and so did the two cheaper-looking alternatives (a band
+        // way moved its gradient by 4.5 % (the C-harness test caught it).  Evaluated for both pixels two-wide;
+        // +14 us per view over two v_exp_f32 -- and so did the two cheaper-looking alternatives (a band
         // test around the threshold with the exact function inline or out of line in the rare branch).
         f2 G;
         if (FAST) {      // VR_FLAG_FAST_EXP: the instruction the forward of this view used
@@ -374,7 +374,7 @@ __device__ __forceinline__ void bwd_chunk_trips(const int lane, const int e, con
         group_prefix_mul_x2<ROWS>(pa, pb);                               // prod over entries >= mine
         const f2 Tl = Tc * (f2){bwd_rcp<DET>(pa), bwd_rcp<DET>(pb)};   // T in front of my splat
         const f2 wgt = a_eff * Tl;
-        // <attr, g> in two independent chains (a dependent v_pk_fma_f32 costs an extra wait state)
+        // <attr, g> in two independent chains
         f2 u0 = f2_splat(at[0]) * g[0], u1 = f2_splat(at[1]) * g[1];
         f2 u;
         if (!no_extra) {
@@ -410,7 +410,7 @@ __device__ __forceinline__ void bwd_chunk_trips(const int lane, const int e, con
             //   conic:   dA += -1/2 a dx^2   dB += -a dx dy   dC += -1/2 a dy^2
             //   mean2D:  dx += -a (A dx + B dy)   dy += -a (C dy + B dx)
             // the factors -1/2 and -1 belong to the SPLAT, i.e. to the lane: sum(a dx dx), sum(a dx dy),
-            // sum(a dy dy), sum(a (A dx + B dy)), sum(a (C dy + B dx)) are accumulated here (12 packed operations
+            // sum(a dy dy), sum(a (A dx + B dy)), sum(a (C dy + B dx)) are accumulated here (12 two-wide operations
             // instead of 20) and the signs applied once per entry at the flush.  (The conic cannot be pulled out of
             // the mean2D sums as well: A sum(a dx) + B sum(a dy) cancels AFTER the sums were rounded, and for edge-on
             // discs that lost two digits -- the C-harness test caught rows off by 2 %.)
@@ -432,7 +432,7 @@ __device__ __forceinline__ void bwd_chunk_trips(const int lane, const int e, con
 
 // NO_DEPTH (round 6): no upstream gradient on the depth image (dL_ddepth == NULL: VEGS' losses reach colour, cov_quat and
 // cov_scale only, train.py:152-168) -- its channel's terms, fma(depth_s, 0, u) in the <attr, g> chain and fma(w, 0, acc) in the
-// accumulators, are the identity for every finite depth and are left out: bit-identical sums, two packed instructions fewer
+// accumulators, are the identity for every finite depth and are left out: bit-identical sums, two two-wide operations fewer
 // per trip.
 template <bool NO_EXTRA, bool DET, bool FAST, bool NO_DEPTH = false>
 __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(4, 4)))
@@ -510,7 +510,7 @@ k_seg_bwd(Camera cam, const int2* __restrict__ ranges, const uint32_t* __restric
     const int seg_lo = c.sl * SEG;       // first list entry (tile-relative) of this segment
     // Per-pixel record in LDS, interleaved by PIXEL PAIR (a = even pixel, b = odd pixel of the strip): the
     // pixel loop reads it back as wave-uniform broadcasts (LDS pipe, not 16 v_readlane on the VALU pipe) and
-    // gets every quantity as a ready-made (a,b) register pair for packed fp32 math.  float4 slots:
+    // gets every quantity as a ready-made (a,b) register pair.  float4 slots:
     //   0 {px_a px_b py_a py_b}  1 {bg_a bg_b g0_a g0_b}  2 {g1 g2}  3 {g3 g4}  4 {g5 g6}  5 {g7 g8}
     //   6 {g9 g10}  7 {Tcar_a Tcar_b Scar_a Scar_b} -- the two carries, updated in place by lane 63.
     // SLOT-MAJOR, pix[slot][pair], and written as whole float4s by the EVEN lanes (the odd pixel's values come over DPP):

@@ -1012,9 +1012,8 @@ k_seg_blend(Camera cam, const int2* __restrict__ ranges, const uint32_t* __restr
             const float4 cc = lds[2][i];  // r g b qw
             const float4 d = lds[3][i];   // qx qy qz s0
             const float2 e2 = *reinterpret_cast<const float2*>(&lds[4][i]);  // s1 s2
-            // the eleven channel sums as the record lays the attributes out: five adjacent pairs (packed fma straight
-            // from the loaded registers -- summed channel by channel the compiler packed them too, after five register
-            // moves per entry) and the depth; each sum is the same fma as before
+            // the eleven channel sums as the record lays the attributes out: five adjacent pairs, straight from the
+            // loaded registers, and the depth; each sum is the same fma as before
             const f2 w2 = f2_splat(wgt);
             Cp[0] = f2_fma((f2){cc.x, cc.y}, w2, Cp[0]);   // r g
             Cp[1] = f2_fma((f2){cc.z, cc.w}, w2, Cp[1]);   // b qw

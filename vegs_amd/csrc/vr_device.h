@@ -175,8 +175,8 @@ __device__ __forceinline__ void wave_copy_from_lds(float* __restrict__ dst, cons
     }
 }
 
-// ---- packed fp32 (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32 process two floats per lane per issue):
-// two-wide helpers for the compositing arithmetic of the backward pass
+// ---- two-wide helpers for the compositing arithmetic of the backward pass (scalar instructions, one per half: the build
+// leaves v_pk_*_f32 out, vegs_amd/build.py)
 typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f2 f2_splat(float v) { f2 r = {v, v}; return r; }
 __device__ __forceinline__ f2 f2_fma(f2 a, f2 b, f2 c) { return __builtin_elementwise_fma(a, b, c); }
