@@ -766,9 +766,8 @@ def main():
                      "frac": round(valu_insts / (ms_k * 1e-3) / 1e9 / VALU_PEAK_GINST, 4),
                      "measured_issue_peak_ginst_per_s": VALU_MEASURED_GINST,
                      "frac_of_measured_issue_peak": round(valu_insts / (ms_k * 1e-3) / 1e9 / VALU_MEASURED_GINST, 4),
-                     "note": "instructions, not issue slots: a packed fp32 instruction takes two slots and a transcendental "
-                             "~3.5 (profiles/tools/ubench/pk_rate.hip); with ~40 % of this kernel's instructions packed and four "
-                             "reciprocals per trip its stream is ~230 us of pure issue (HISTORY.md section 14)"},
+                     "note": "instructions, not issue slots: a transcendental takes ~3.5 (profiles/tools/ubench/pk_rate.hip), four "
+                             "reciprocals per trip; the build has no packed fp32 instructions, which would take two slots"},
                  "l2_atomics": None if flushes is None else {
                      "kernel": kern, "flushes_per_view": round(flushes), "atomics_per_view": round(17 * flushes),
                      "achieved_gatomics_per_s": round(17 * flushes / (ms_k * 1e-3) / 1e9, 2) if ms_k > 0 else None,
