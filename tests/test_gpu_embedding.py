@@ -244,6 +244,37 @@ def test_shapes_and_layouts():
     assert torch.equal(embedding.lookup(whole[:, 0, 0].contiguous(), flat.clamp(min=0)), whole[:, 0, 0][flat.clamp(min=0)])
 
 
+@pytest.mark.parametrize("n", [100, 5000, 30000])
+@pytest.mark.parametrize("how", ["recomputed", "offloaded"])
+@pytest.mark.parametrize("by_row", [False, True])
+def test_saved_tensors_that_move(n, how, by_row):
+    """What the gradient reads comes back from the hooks on saved tensors, not from where the forward had it: there something
+    else stands by then.  Whole numbers: every sum is exact."""
+    from torch.utils.checkpoint import checkpoint
+    from vegs_amd import embedding
+    table, ids, scale, g = _inputs(n, 301, 12, "holes", scale="row" if by_row else 2.0, whole=True)
+    table.requires_grad_(True)
+    wanted = [table] + ([scale.requires_grad_(True)] if by_row else [])
+
+    def rows():
+        # ids, scales and a table that live no longer than the call, the table as rows with a gap
+        wide = torch.zeros((301, 16), device=DEV)
+        wide[:, :12] = table
+        return embedding.lookup(wide[:, :12], ids + 0, 1.0 * scale if by_row else scale)
+
+    want = torch.autograd.grad(rows(), wanted, g)
+    if how == "recomputed":
+        out = checkpoint(rows, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            out = rows()
+    over = [torch.full((k,), 3, dtype=torch.int64, device=DEV) for k in (n, n // 2, 301 * 8, 301 * 6) for _ in range(8)]
+    for x, y in zip(torch.autograd.grad(out, wanted, g), want):
+        assert torch.equal(x, y)
+    _check(table.detach(), ids, scale.detach() if by_row else scale, g, exact=True)
+    del over
+
+
 def test_only_one_of_the_gradients_is_wanted():
     from vegs_amd import embedding
     table, ids, scale, g = _inputs(300, 30, 45, "holes", seed=11)

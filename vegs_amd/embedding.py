@@ -66,18 +66,19 @@ def _forward(arguments, shape, dtype, device):
 
 
 def _backward(ctx, g):
-    keep = ctx.saved_tensors                      # (what the arguments point at, as far as it is read)
     device, index = g.device, g.get_device()
     if torch.cuda.current_device() != index:
         with torch.cuda.device(index):
             return _backward(ctx, g)
-    arguments, shape, dtype, ids_shape, n, width = ctx.lookup
+    # (hooks on saved tensors -- recomputation, offloading -- give them back at addresses of their own)
+    rows, flat, scales = ctx.saved_tensors
+    scale, shape, kind, dtype, ids_shape, n, width = ctx.lookup
     want_table, _, want_scale, _, _ = ctx.needs_input_grad
     d_table = d_scale = scratch = None
     nbytes = at_table = at_scale = 0
     lib = _capi._lib or _capi.load()
     if want_table:
-        d_table = torch.empty(shape, dtype=dtype, device=device)
+        d_table = torch.empty(shape, dtype=kind, device=device)
         at_table = d_table.data_ptr()
         nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width)
     if want_scale:
@@ -90,6 +91,8 @@ def _backward(ctx, g):
         g, stride = _row_layout(g, len(ids_shape), width)
     if nbytes:
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    # (the table's values are only read for the gradient of the scales: where that is not wanted, anything of its shape stands for it)
+    arguments, *keep = _arguments(d_table if rows is None else rows, flat, scale if scales is None else scales, width, dtype)
     rc = lib.vr_lookup_backward(arguments, g.data_ptr(), stride, at_table, at_scale, scratch.data_ptr() if nbytes else None, nbytes,
                                 _capi.stream_of(device))
     if rc:
@@ -105,8 +108,7 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, width, dtype):
         arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
-        ctx.lookup = arguments, table.shape, table.dtype, ids.shape, ids.numel(), width
-        # (the table's values are only read again for the gradient of the scales)
+        ctx.lookup = None if scales is not None else scale, table.shape, table.dtype, dtype, ids.shape, ids.numel(), width
         ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, flat, scales)
         return _forward(arguments, ids.shape + table.shape[1:], dtype, table.device)
 
