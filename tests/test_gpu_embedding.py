@@ -345,6 +345,20 @@ def test_more_values_than_31_bits_count():
     assert d[1:rows - 6].abs().max().item() == 0.0
 
 
+def test_more_threads_than_32_bits_count():
+    """The scales' gradient alone takes a wave for each of 67 million entries, the forward a quarter of one.  Whole numbers: exact."""
+    from vegs_amd import embedding
+    n, rows, width = (1 << 26) + 3, 5, 129
+    table = ((torch.arange(rows * width, device=DEV) * 7) % 5 - 2.0).reshape(rows, width)
+    ids = (torch.arange(n, dtype=torch.int32, device=DEV) % (rows + 1))                # one in six: no row
+    scale = (1.0 + torch.arange(n, device=DEV) % 3).float().requires_grad_(True)
+    out = embedding.lookup(table, ids, scale)
+    d, = torch.autograd.grad(out, [scale], out.detach())                              # s |T[id]|^2
+    square = torch.cat((table.square().sum(1), table.new_zeros(1)))
+    assert torch.equal(d, scale.detach() * square[ids.long()])
+    assert torch.equal(out[-7:].detach(), scale.detach()[-7:, None] * torch.cat((table, table.new_zeros(1, width)))[ids[-7:].long()])
+
+
 def test_on_another_stream():
     """Forward and backward run where the caller's stream is; their workspaces are used again at once."""
     side = torch.cuda.Stream()

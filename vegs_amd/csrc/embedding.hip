@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) k_lookup_fwd(LookupArgs a, TO* __restrict
     if (want >= a.width) return;
     // the last lane of a row that is no multiple of V starts early and writes some of its neighbour's columns again
     const long col = want + V <= a.width ? want : (a.width >= V ? a.width - V : 0);
-    const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long wave = ((long)blockIdx.z * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
     const long first = wave * (per * FWD_ENTRIES) + ((threadIdx.x & 63) >> g_shift);
     const TT* table = reinterpret_cast<const TT*>(a.table) + col;
     long row[FWD_ENTRIES];
@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(256) k_lookup_dscale(LookupArgs a, const TO* _
                                                        float* __restrict__ d_row_scale, int g_shift)
 {
     const int G = 1 << g_shift, lane = threadIdx.x & (G - 1);
-    const long i = ((long)blockIdx.x * 256 + threadIdx.x) >> g_shift;
+    const long i = (((long)blockIdx.z * gridDim.x + blockIdx.x) * 256 + threadIdx.x) >> g_shift;
     if (i >= a.n) return;
     const long row = row_of(a, i);
     float acc = 0.0f;
@@ -871,6 +871,14 @@ static Tiling tiling(int64_t n, int64_t width, int v_full)
     return t;
 }
 
+// A grid of `blocks` workgroups by `tiles`.  A launch has fewer than 2^32 threads in x, which 2^24 workgroups of 256 would be:
+// more than 2^20 go on in z.
+static dim3 grid_of(int64_t blocks, int tiles)
+{
+    const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+    return dim3((unsigned)x, (unsigned)tiles, (unsigned)((blocks + x - 1) / x));
+}
+
 static int check_lookup(const VrLookup* l, LookupArgs& a)
 {
     if (!l) { set_error("lookup: arguments are required"); return VR_ERR_INVALID_ARGUMENT; }
@@ -911,7 +919,7 @@ struct Forward {
         constexpr int V = 16 / sizeof(TO);
         const Tiling t = tiling(a.n, a.width, V);
         const long per = 4 * (64 >> t.g_shift) * FWD_ENTRIES;
-        const dim3 grid((unsigned)((a.n + per - 1) / per), t.tiles);
+        const dim3 grid = grid_of((a.n + per - 1) / per, t.tiles);
         if (t.V != V) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO, 1, false>), grid, dim3(256), 0, s, a, (TO*)out, t.g_shift);
         else if (a.n * a.width * (long)sizeof(TO) >= FWD_NT_BYTES)
             hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_fwd<TT, TO, V, true>), grid, dim3(256), 0, s, a, (TO*)out, t.g_shift);
@@ -944,7 +952,7 @@ struct Backward {
                                    dim3(JOIN_THREADS), 0, s, a, q, t.chunks, each);
         }
         if (q.d_row_scale && !fused)
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_dscale<TT, TO, V>), dim3((unsigned)(((a.n << t.g_shift) + 255) / 256)), dim3(256),
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_dscale<TT, TO, V>), grid_of(((a.n << t.g_shift) + 255) / 256, 1), dim3(256),
                                0, s, a, reinterpret_cast<const TO*>(q.grad), q.grad_stride, q.d_row_scale, t.g_shift);
     }
     template <typename TT, typename TO>
