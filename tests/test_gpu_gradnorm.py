@@ -187,6 +187,21 @@ def test_a_bound_of_zero_and_of_infinity():
     assert (g == 0).all()
 
 
+def test_one_gradient_of_more_values_than_31_bits_count():
+    """3, 4 and 12 at the borders where an offset would be cut: the norm is 13, half of it the factor one half of powers of two."""
+    from vegs_amd import optim
+    n = 2 ** 31 + 2 ** 17 + 5
+    p = torch.empty(n, dtype=torch.bfloat16, device=DEV)
+    p.grad = torch.zeros_like(p)
+    places = (0, 2 ** 31 - 1, 2 ** 31, n - 1)
+    for at, x in zip(places, (3.0, 4.0, 0.0, 12.0)):
+        p.grad[at] = x
+    assert optim.grad_norm(p).item() == 13.0 and optim.grad_norm(p, math.inf).item() == 12.0
+    assert optim.clip_grad_norm_(p, 6.5).item() == 13.0
+    assert [p.grad[at].item() for at in places] == [1.5, 2.0, 0.0, 6.0]           # (6.5 / (13 + 1e-6) rounds to a half of them in 8 bits)
+    assert p.grad.count_nonzero().item() == 3
+
+
 def test_a_gradient_met_twice_counts_once():
     from vegs_amd import optim
     g, = _make([(5000,)])
@@ -379,6 +394,20 @@ def test_factored_gradients_in_the_norm_and_the_step(P, deg, views, split):
     own = optim.adam_step_sh_factored(opt, ps[0], ps[1] if split else None, means, campos, factors, deg, scale, max_grad_norm=1e9)
     want = _norm64(list(dense) if split else [dense])
     assert abs(own.item() - want) <= 2.0 ** -24 * 1.01 * want
+
+
+def test_factored_gradients_of_as_many_points_as_31_bits_count():
+    """Degree 0: the row is scale x 0.28209479 x the factor, wherever its point stands.  One fp32 rounding of the constant, of each
+    of the two products and of the norm itself: 4 x 2^-24."""
+    from vegs_amd import optim
+    P = 2 ** 31 - 1
+    means, factors = torch.zeros((P, 3), device=DEV), torch.zeros((1, P, 3), device=DEV)
+    for at, x in ((0, 3.0), (2 ** 31 - 2 ** 18 - 2, 4.0), (P - 1, 12.0)):
+        factors[0, at, at % 3] = x
+    sh = [(means, torch.ones((1, 3), device=DEV), factors, 0, 0.5)]
+    for norm_type, want in ((2.0, 13.0), (math.inf, 12.0)):
+        want *= 0.5 * 0.28209479177387814
+        assert abs(optim.grad_norm([], norm_type, sh_factors=sh).item() - want) <= 4.01 * 2.0 ** -24 * want
 
 
 @pytest.mark.parametrize("n_boxes,factored", [(0, False), (0, True), (2, False), (2, True)])

@@ -127,11 +127,11 @@ __global__ void __launch_bounds__(256) k_sh_grad_norm(ShFactorArgs a, double* __
     using A = typename Acc<MAX>::type;
     __shared__ A lds[4];
     A acc = 0;
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < a.P; i += gridDim.x * 256) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < a.P; i += gridDim.x * 256) {
         float g[SHF_ROW_MAX];
 #pragma unroll
         for (int q = 0; q < SHF_ROW_MAX; ++q) g[q] = 0.0f;
-        sh_row_from_factors(a, i, g);
+        sh_row_from_factors(a, (int)i, g);
 #pragma unroll
         for (int q = 0; q < SHF_ROW_MAX; ++q) acc = norm_add(acc, a.scale * g[q]);
     }
