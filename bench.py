@@ -42,6 +42,12 @@ def _trace(msg):
         print(f"[bench trace] {msg}", file=sys.stderr, flush=True)
 
 
+def collected_here(args):
+    """Whether this run is of the workload whose counters profiles/pmc_traffic.json holds: the defaults'."""
+    return (args.workload == "c3" and args.gaussians in (0, 2_000_000) and (args.width, args.height) == (1376, 376)
+            and args.disc_scale == 1.0)
+
+
 def profile_figures(kern, sources):
     """(HBM traffic bytes per launch, VALU wave-instructions per launch, provenance) of `kern` from the committed PMC
     profile (profiles/pmc_traffic.json) -- or (None, None, reason) when a source file of that kernel has changed since
@@ -755,7 +761,8 @@ def main():
     achieved = bytes_k / (ms_k * 1e-3) / 1e9 if ms_k > 0 else 0.0
     # (the kernel's own sources AND everything upstream that shapes its work: lists, masks, records)
     traffic, valu_insts, traffic_from = profile_figures(kern, ("render_bwd.hip", "vr_segment.h", "vr_device.h", "render_fwd.hip",
-                                                               "binning.hip", "preprocess.hip"))
+                                                               "binning.hip", "preprocess.hip")) if collected_here(args) else (
+        None, None, "collected on the default workload only")
     # secondary ceilings (reported, not graded): VALU issue -- wave-level VALU instructions of the kernel (SQ
     # counters of the committed profile) against 1024 SIMDs x 2.4 GHz / 2 cycles per wave64 instruction -- and the L2
     # atomics of the backward: 17 fp32 atomics per (list entry, 8x8 region) flush, counted on the device per view
@@ -835,7 +842,7 @@ def main():
                      "stages": stage_frac,
                      "whole_view_alg_bytes": round(b_alg),
                      # (counter bytes of every kernel of one view, committed profile; null while any kernel source is newer)
-                     "whole_view_traffic": whole_view_traffic(),
+                     "whole_view_traffic": whole_view_traffic() if collected_here(args) else None,
                      "whole_view_frac": round(b_alg / t_view / 1e9 / HBM_PEAK_GBS, 5),
                      "whole_view_frac_on_reference_lists": round(b_alg_ref / t_view / 1e9 / HBM_PEAK_GBS, 5)},
     }
