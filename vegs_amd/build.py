@@ -42,9 +42,9 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-# Reproducer builds (profiles/experiments/README.md): the same sources with a -D switch, into their own library beside the
+# Comparison builds (profiles/experiments/README.md): the same sources with a -D switch, into their own library beside the
 # product one -- loaded only when VEGS_LIB names it (vegs_amd/_capi.py).  Never built by build() without --variant.
-VARIANTS = {"early": ["-DVR_EARLY_SH"], "nopack": ["-DVR_BWD_PACK_TAILS=0", "-DVR_BWD_PREFETCH=0"],
+VARIANTS = {"nopack": ["-DVR_BWD_PACK_TAILS=0", "-DVR_BWD_PREFETCH=0"],
             "nopref": ["-DVR_BWD_PREFETCH=0"]}
 
 

@@ -85,28 +85,6 @@ k_preprocess(Camera cam, int P, const float* __restrict__ means3D, const float* 
         pz3 = means3D[3 * (size_t)i + 2];
         xform43(cam.view, px3, py3, pz3, t0, t1, t2);
     }
-#ifdef VR_EARLY_SH
-    // REPRODUCER BUILD ONLY (python -m vegs_amd.build --variant early; profiles/experiments/README.md, round 5/6): the SH rows
-    // of every Gaussian in front of the near plane requested a round trip earlier.  Same results, different timing and
-    // register pressure: the build whose bench runs ended in a memory fault in k_emit_scan.
-    float4 eA[6], eB[6];
-    unsigned long long front_rows = 0ull;
-    if (HALF == 1 && shs) {
-        front_rows = __ballot(in_range && t2 > NEAR_Z);
-        if (front_rows != 0ull) {
-            const size_t wf = (size_t)(blockIdx.x * blockDim.x + w * 64);
-            const float4* s4 = reinterpret_cast<const float4*>(shs + wf * 48);
-#pragma unroll
-            for (int j = 0; j < 6; ++j) {
-                const int v = lane + 64 * j, r = v / 6, c = v - r * 6;
-                if ((front_rows >> r) & 1ull) {
-                    eA[j] = nt_load4(&s4[r * 12 + c]);
-                    eB[j] = nt_load4(&s4[r * 12 + 6 + c]);
-                }
-            }
-        }
-    }
-#endif
     if (in_range) {
         if (t2 > NEAR_Z) {
             float h0, h1, h2;
@@ -242,9 +220,7 @@ k_preprocess(Camera cam, int P, const float* __restrict__ means3D, const float* 
                 // Both halves of the wave's rows are requested at once (12 loads per lane in flight, rows of culled Gaussians
                 // left out); the second half waits in registers while the first is evaluated.  (Requesting them a round trip
                 // EARLIER -- for every Gaussian in front of the near plane, before the covariance and the tile test -- measured
-                // slower, 0.152 against 0.148 ms.  That build's bench runs once ended in a memory fault in k_emit_scan on one box
-                // (garbage ids out of the depth sort); it is kept as the reproducer build -DVR_EARLY_SH above and has not
-                // faulted since, with or without the depth sort's post-mortem: profiles/experiments/README.md, round 6.)
+                // slower, 0.152 against 0.148 ms.)
                 const float* rows = HALF == 1 ? shs + wave_first * 48 : shs_tail + (wave_first - (size_t)tail_start) * 48;
                 const float4* src4 = reinterpret_cast<const float4*>(rows);
                 float4 tA[6], tB[6];
@@ -255,9 +231,6 @@ k_preprocess(Camera cam, int P, const float* __restrict__ means3D, const float* 
                     const int v = lane + 64 * j, r = v / 6, c = v - r * 6;
                     ok[j] = (vis_rows >> r) & 1ull;
                     at[j] = r * (SH_HALF_STRIDE / 4) + c;
-#ifdef VR_EARLY_SH
-                    if (HALF == 1) { tA[j] = eA[j]; tB[j] = eB[j]; continue; }
-#endif
                     if (ok[j]) {
                         tA[j] = nt_load4(&src4[r * 12 + c]);
                         tB[j] = nt_load4(&src4[r * 12 + 6 + c]);
