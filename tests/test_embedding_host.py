@@ -75,3 +75,29 @@ def test_rows_that_lie_apart_are_taken_as_they_are():
         assert copy.is_contiguous() and stride == other[0].numel()
     copy, stride = embedding._row_layout(part, 2, 4)       # two leading dimensions: not one stride
     assert copy.is_contiguous() and stride == 4
+
+
+_EMPTY = r"""
+import sys
+sys.path.insert(0, %r)
+import ctypes as C
+from vegs_amd import _capi
+lib, some = _capi.load(), 1 << 20
+for dtype, width in ((0, 3), (0, 256), (0, 257), (0, 1000), (1, 513), (2, 1 << 22)):
+    empty = _capi.VrLookup(some, None, None, 0, 7, width, width, dtype, dtype, 0, 1.0)
+    for d_table, d_scale in ((some, some), (some, None), (None, some), (None, None)):
+        lib.vr_lookup_backward(C.byref(empty), None, width, d_table, d_scale, None, 0, None)
+    print(dtype, width, lib.vr_lookup_backward(C.byref(empty), None, width, None, some, None, 0, None), flush=True)
+"""
+
+
+def test_gradients_of_no_entries_do_not_end_the_process():
+    """In a process of its own that sees no GPU (the addresses are made up: there the launch that clears the gradient fails)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _EMPTY % root], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, HIP_VISIBLE_DEVICES="-1", ROCR_VISIBLE_DEVICES="-1"))
+    assert r.returncode == 0, (r.returncode, r.stdout[-500:], r.stderr[-2000:])
+    assert [line.split()[2] for line in r.stdout.split("\n") if line] == ["0"] * 6       # the scales' gradient of no entries: nothing to do

@@ -455,3 +455,18 @@ def test_codebook_through_the_rasterizer_into_a_clipped_step(by_row):
         # a first step moves every value by lr g / (|g| + eps): the factor cancels but for eps, 1e-8 beside clipped gradients:
         # the step's own roundings (at most 16 u) plus eps' share of an 8 u error, and the value's rounding
         assert ((p.detach().double().cpu() - q.detach()).abs() <= 24 * u * lr + u * q.detach().abs() * 1.01).all()
+
+
+@pytest.mark.parametrize("dtype,width", [(0, 3), (0, 256), (0, 257), (0, 1000), (1, 600)])
+def test_no_entries_at_the_c_entry(dtype, width):
+    """The table's gradient is zeros, and the scales' gradient, which has no elements, is left alone."""
+    import ctypes as C
+    from vegs_amd import _capi
+    table = torch.ones(7, width, device=DEV, dtype=(F32, BF16)[dtype])
+    d_table, d_scale = torch.full_like(table, 3.0), torch.full((4,), 5.0, device=DEV)
+    empty = _capi.VrLookup(table.data_ptr(), None, None, 0, 7, width, width, dtype, dtype, 0, 1.0)
+    stream = torch.cuda.current_stream().cuda_stream
+    for scales in (d_scale.data_ptr(), None):
+        d_table.fill_(3.0)
+        assert _capi.load().vr_lookup_backward(C.byref(empty), None, width, d_table.data_ptr(), scales, None, 0, stream) == 0
+        assert (d_table == 0).all() and (d_scale == 5.0).all()

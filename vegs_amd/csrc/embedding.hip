@@ -875,7 +875,7 @@ static Tiling tiling(int64_t n, int64_t width, int v_full)
 // more than 2^20 go on in z.
 static dim3 grid_of(int64_t blocks, int tiles)
 {
-    const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+    const int64_t x = blocks < 1 ? 1 : blocks < (1 << 20) ? blocks : 1 << 20;
     return dim3((unsigned)x, (unsigned)tiles, (unsigned)((blocks + x - 1) / x));
 }
 
@@ -1020,7 +1020,8 @@ extern "C" int vr_lookup_backward(const VrLookup* lookup, const void* grad, int6
     if (d_table && a.n > SMALL && (!scratch || ((uintptr_t)scratch & 255) || scratch_bytes < vr_lookup_scratch_bytes(a.n, a.rows, a.width)))
         { set_error("lookup: the table's gradient needs vr_lookup_scratch_bytes of scratch, 256-byte aligned"); return VR_ERR_INVALID_ARGUMENT; }
     if (a.rows == 0) d_table = nullptr;
-    if (!d_table && (!d_row_scale || a.n == 0)) return VR_OK;
+    if (a.n == 0) d_row_scale = nullptr;                // (without entries there is only the table's gradient to clear)
+    if (!d_table && !d_row_scale) return VR_OK;
     hipStream_t s = (hipStream_t)stream;
     SumArgs q{nullptr, nullptr, nullptr, grad, (long)grad_stride, d_table, d_row_scale, nullptr, 0, 0};
     if (d_table && a.n > SMALL) {
