@@ -69,7 +69,8 @@ int vr_grad_norm(const VrGradTensor* tensors, int32_t count, const VrShGradFacto
 
 /* In place, for every element: g *= min(1, max_norm / (norm[0] + 1e-6)), the product in fp32 and rounded once to the
  * gradient's type.  A factor of exactly one writes nothing; a NaN norm makes every element NaN and an infinite one gives
- * zeros (NaN where the element itself is infinite), as torch.nn.utils.clip_grad_norm_ does.  max_norm >= 0. */
+ * zeros (NaN where the element itself is infinite), as torch.nn.utils.clip_grad_norm_ does.  max_norm >= 0.  Tensors that
+ * share memory are refused (VR_ERR_INVALID_ARGUMENT), here and by vr_clip_grad_norm: two workgroups would scale it. */
 int vr_clip_grads(const VrGradTensor* tensors, int32_t count, const float* norm, float max_norm, void* stream);
 
 /* vr_grad_norm and vr_clip_grads in a row; a handful of small tensors takes one launch for both. */

@@ -442,3 +442,51 @@ def test_trainer_clips_all_its_optimizers_by_one_norm(n_boxes, factored):
     for k in names:                     # both sides (1 - beta1) times a gradient: 2 u and 8 u + 2 u
         want = m0[k].double() * c
         assert ((m1[k].double() - want).abs() <= 12 * 2.0 ** -24 * want.abs() + 2.0 ** -148).all(), k
+
+
+def test_gradients_that_begin_at_one_address():
+    """b[:n] and b[::2] of one buffer: other elements, so both enter the norm; each value in memory is scaled once."""
+    from vegs_amd import optim
+    n = 4000
+    b, = _make([(2 * n,)], seed=3)
+    before = b.clone()
+    dense, apart = _param(b[:n]), torch.empty(n, device=DEV)
+    apart.grad = b[::2]
+    want = _norm64([before[:n], before[::2]])
+    assert abs(optim.grad_norm([dense, apart]).item() - want) <= 2.0 ** -24 * 1.01 * want
+    opts = [optim.Adam([torch.nn.Parameter(torch.zeros(n, device=DEV))]) for _ in range(2)]
+    for o, g in zip(opts, (b[:n], b[::2])):
+        o.param_groups[0]["params"][0].grad = g
+    assert abs(optim.step_many(opts, max_grad_norm=1.0).item() - want) <= 2.0 ** -24 * 1.01 * want
+    for params in ([dense, apart], [apart, dense]):
+        b.copy_(before)
+        norm = optim.clip_grad_norm_(params, 0.25 * want)
+        assert abs(norm.item() - want) <= 2.0 ** -24 * 1.01 * want
+        held = torch.zeros(2 * n, dtype=torch.bool, device=DEV)
+        held[:n] = held[::2] = True
+        _check_clipped([before[held]], [b[held]], want, 0.25 * want)
+        assert torch.equal(b[~held], before[~held])
+
+
+def test_columns_of_one_buffer_are_clipped_as_they_are():
+    from vegs_amd import optim
+    b, = _make([(700, 9)], seed=4)
+    before = b.clone()
+    left, right = torch.empty(700, 3, device=DEV), torch.empty(700, 6, device=DEV)
+    left.grad, right.grad = b[:, :3], b[:, 3:]
+    want = _norm64([before])
+    norm = optim.clip_grad_norm_([left, right], 0.5 * want)
+    assert abs(norm.item() - want) <= 2.0 ** -24 * 1.01 * want
+    _check_clipped([before], [b], want, 0.5 * want)
+
+
+@pytest.mark.parametrize("error_if_nonfinite", [False, True])
+def test_gradients_that_share_a_part_of_their_memory_are_refused(error_if_nonfinite):
+    from vegs_amd import optim
+    b, = _make([(9000,)], seed=5)
+    before = b.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        optim.clip_grad_norm_([_param(b[:6000]), _param(b[5999:])], 1.0, error_if_nonfinite=error_if_nonfinite)
+    assert torch.equal(b, before)
+    want = _norm64([before[:6000], before[5999:]])
+    assert abs(optim.grad_norm([_param(b[:6000]), _param(b[5999:])]).item() - want) <= 2.0 ** -24 * 1.01 * want

@@ -106,3 +106,28 @@ def test_sparse_gradients_are_refused():
         optim.grad_norm([p])
     with pytest.raises(ValueError, match="dense"):
         optim.clip_grad_norm_([p], 1.0)
+
+
+def test_gradients_are_told_apart_by_their_elements():
+    b = torch.zeros(12)
+    assert len(optim._once([b[:4], b[::2][:4]])) == 2             # one address and one number of elements, other elements
+    assert len(optim._once([b[:4], b[:4], b[:4].reshape(2, 2), b[:4].reshape(2, 2).t()])) == 1
+    assert len(optim._once([b[::2], b[::2], b[::3][:4], b[::2][:4]])) == 3
+    assert len(optim._once([b[:4], b.view(torch.int32)[:4]])) == 2
+
+
+def test_c_entries_refuse_to_scale_shared_memory():
+    """(Made-up addresses: nothing is launched for a refused call.)"""
+    lib = _capi.load()
+    some = 1 << 20
+
+    def table(*entries):
+        return (C.c_int64 * (3 * len(entries)))(*[x for e in entries for x in e]), len(entries)
+
+    many = [(some + 4096 * i, 1024, 0) for i in range(300)]
+    for entries in ([(some, 8, 0), (some, 8, 0)], [(some, 8, 0), (some + 28, 1, 0)], [(some + 28, 5, 0), (some, 8, 0)],
+                    [(some, 9, 1), (some + 16, 4, 0)], [(some, 100, 0), (some + 1000, 5, 0), (0, 0, 0), (some + 200, 3, 1)],
+                    many + [(some + 4096 * 200 + 4092, 1, 0)]):
+        t, n = table(*entries)
+        for rc in (lib.vr_clip_grads(t, n, some, 1.0, None), lib.vr_clip_grad_norm(t, n, 2, 1.0, some, some, None)):
+            assert rc == -1 and b"share memory" in lib.vr_last_error()

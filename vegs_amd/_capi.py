@@ -307,6 +307,9 @@ class VegsRastError(RuntimeError):
     pass
 
 
+INVALID_ARGUMENT = -1           # VR_ERR_INVALID_ARGUMENT
+
+
 def check(rc):
     if rc != 0:
         raise VegsRastError(f"libvegsrast error {rc}: {load().vr_last_error().decode()}")

@@ -12,6 +12,9 @@
 #include "vr_sh_factors.h"
 #include "vr_types.h"
 
+#include <algorithm>
+#include <new>
+
 namespace vr {
 
 constexpr int GN_MAX_T = 128;              // tensors per launch: the table is a kernel argument, 128 x 24 B of its 4 KB
@@ -261,6 +264,31 @@ static int check_grads(const VrGradTensor* t, int32_t count)
     return VR_OK;
 }
 
+// Whether no two of the tensors share memory: workgroups scale units of different tensors side by side, and an element that two
+// of them hold would be read, multiplied and written by both.
+static int check_apart(const VrGradTensor* t, int32_t count)
+{
+    struct Range { uintptr_t begin, end; int at; };
+    Range few[GN_MAX_T];
+    Range* r = count <= GN_MAX_T ? few : new (std::nothrow) Range[count];
+    if (!r) { set_error("clip: no memory for a list of %d tensors", count); return VR_ERR_ALLOC; }
+    int n = 0;
+    for (int i = 0; i < count; ++i)
+        if (t[i].n > 0) {
+            const uintptr_t at = (uintptr_t)t[i].data;
+            r[n++] = Range{at, at + (uintptr_t)t[i].n * (t[i].dtype == VR_F32 ? 4 : 2), i};
+        }
+    std::sort(r, r + n, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    int rc = VR_OK;
+    for (int i = 1; i < n && rc == VR_OK; ++i)
+        if (r[i].begin < r[i - 1].end) {
+            set_error("clip: tensors %d and %d share memory", std::min(r[i - 1].at, r[i].at), std::max(r[i - 1].at, r[i].at));
+            rc = VR_ERR_INVALID_ARGUMENT;
+        }
+    if (r != few) delete[] r;
+    return rc;
+}
+
 // the next launch's table: up to GN_MAX_T non-empty tensors from `first` on; returns the first one not consumed
 static int fill_grads(const VrGradTensor* t, int first, int count, GradArgs& a)
 {
@@ -377,6 +405,7 @@ extern "C" int vr_clip_grads(const VrGradTensor* tensors, int32_t count, const f
 {
     if (int rc = check_grads(tensors, count)) return rc;
     if (!norm || !(max_norm >= 0.0f)) { set_error("clip: needs a norm and max_norm >= 0"); return VR_ERR_INVALID_ARGUMENT; }
+    if (int rc = check_apart(tensors, count)) return rc;
     return clip_grads(tensors, count, norm, max_norm, (hipStream_t)stream);
 }
 
@@ -385,6 +414,7 @@ extern "C" int vr_clip_grad_norm(const VrGradTensor* tensors, int32_t count, int
 {
     if (!(max_norm >= 0.0f)) { set_error("clip: max_norm must not be negative or NaN"); return VR_ERR_INVALID_ARGUMENT; }
     if (int rc = check_norm(tensors, count, nullptr, 0, norm_type, norm, scratch)) return rc;
+    if (int rc = check_apart(tensors, count)) return rc;
     return norm_type == 2 ? grad_norm<false>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, true, max_norm)
                           : grad_norm<true>(tensors, count, nullptr, 0, norm, (double*)scratch, (hipStream_t)stream, true, max_norm);
 }

@@ -88,8 +88,7 @@ _ADAM = struct.Struct("4Qqdqd")           # VrAdamTensor
 
 
 def _grads_of(parameters):
-    """The gradients of `parameters` -- a tensor, an optimizer, or an iterable of either -- each one once.  (Two launches of
-    the scaling's workgroups on one gradient would race.)"""
+    """The gradients of `parameters` -- a tensor, an optimizer, or an iterable of either -- each one once."""
     if isinstance(parameters, (torch.Tensor, torch.optim.Optimizer)):
         parameters = [parameters]
     grads = []
@@ -102,10 +101,15 @@ def _grads_of(parameters):
 
 
 def _once(grads):
+    """Gradients that are the same elements of the same memory, once: the order of the dimensions tells two that fill their memory
+    not apart, but their strides tell two others that begin at one address."""
+    seen = {}
     for g in grads:
         if g.layout is not torch.strided:
             raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.layout})")
-    return list({(g.data_ptr(), g.numel()): g for g in grads}.values())
+        at, n = g.data_ptr(), g.numel()
+        seen[(at, n, g.dtype) if _dense(g) else (at, n, g.dtype, g.shape, g.stride())] = g
+    return list(seen.values())
 
 
 def _dense(t):
@@ -194,7 +198,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """torch.nn.utils.clip_grad_norm_ on the GPU: scales the gradients of `parameters` (a tensor, an optimizer, or an iterable
     of either) in place by min(1, max_norm / (norm + 1e-6)) and returns their norm from before, a 0-dim float32 tensor.
     The norm is grad_norm()'s.  Gradients below the bound are not written at all; a NaN norm makes all of them NaN, as in
-    torch; error_if_nonfinite=True waits for the norm and raises before anything is scaled.  `foreach` has no effect (there
+    torch.  Two gradients that share a part of their memory are refused, unless the elements of one do not fill their memory:
+    then each value in memory is scaled once, and enters the norm once for each gradient that holds it.
+    error_if_nonfinite=True waits for the norm and raises before anything is scaled.  `foreach` has no effect (there
     is one path).  step_many(max_grad_norm=...) clips inside the Adam step instead and leaves the gradients alone."""
     max_norm, kind = _check_max_norm(max_norm), _norm_kind(norm_type)
     grads = _grads_of(parameters)
@@ -218,9 +224,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             if not math.isfinite(norm.item()):
                 raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is not finite, so they cannot be "
                                    "clipped; error_if_nonfinite=False scales them all the same")
-            _capi.check(lib.vr_clip_grads(table, len(grads), norm.data_ptr(), max_norm, stream))
+            rc = lib.vr_clip_grads(table, len(grads), norm.data_ptr(), max_norm, stream)
         else:
-            _capi.check(lib.vr_clip_grad_norm(table, len(grads), kind, max_norm, norm.data_ptr(), scratch.data_ptr(), stream))
+            rc = lib.vr_clip_grad_norm(table, len(grads), kind, max_norm, norm.data_ptr(), scratch.data_ptr(), stream)
+    if rc == _capi.INVALID_ARGUMENT:                  # (what is left for the library to refuse: shared memory)
+        raise ValueError(lib.vr_last_error().decode())
+    _capi.check(rc)
     for g, copy in copies:
         g.copy_(copy)
     return norm
