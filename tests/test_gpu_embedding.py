@@ -470,3 +470,24 @@ def test_no_entries_at_the_c_entry(dtype, width):
         d_table.fill_(3.0)
         assert _capi.load().vr_lookup_backward(C.byref(empty), None, width, d_table.data_ptr(), scales, None, 0, stream) == 0
         assert (d_table == 0).all() and (d_scale == 5.0).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor requires no gradient and has an address like any other: its tangent may not get lost on the way."""
+    import torch.autograd.forward_ad as fwd
+    from vegs_amd import embedding
+    table, ids, scale, _ = _inputs(50, 9, 5, "holes", seed=2)
+    want = embedding.lookup(table, ids, scale)
+    with fwd.dual_level():
+        dual, dual_scale = fwd.make_dual(table, torch.ones_like(table)), fwd.make_dual(scale, torch.ones_like(scale))
+        for t, s in ((dual, None), (dual, 2.0), (dual, scale), (table, dual_scale), (dual, dual_scale)):
+            for mode in (torch.enable_grad(), torch.no_grad()):
+                with mode, pytest.raises(NotImplementedError, match="jvp"):
+                    embedding.lookup(t, ids, s)
+        assert torch.equal(embedding.lookup(table, ids, scale), want)             # no tangent: nothing to refuse
+        with torch.no_grad():
+            out = embedding.lookup(table.clone().requires_grad_(True), ids, scale)
+            assert torch.equal(out, want) and not out.requires_grad
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: embedding.lookup(t, ids, scale), (table,), (table,))
+    assert torch.equal(embedding.lookup(table, ids, scale), want)

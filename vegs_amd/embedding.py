@@ -13,6 +13,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -127,7 +128,7 @@ def lookup(table, ids, scale=None, dtype=None):
 
     The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in float32, in an order
     that the sizes and ids fix, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same
-    bits every time."""
+    bits every time.  Forward-mode differentiation is refused, as by every operator of this package."""
     if not isinstance(table, torch.Tensor) or not table.is_cuda:
         raise ValueError("table must be a GPU tensor (there is no CPU path)")
     shape, kind, device = table.shape, table.dtype, table.device
@@ -152,7 +153,8 @@ def lookup(table, ids, scale=None, dtype=None):
         dtype = kind
     elif dtype != kind and dtype != torch.float32:
         raise ValueError(f"the result has the table's type or float32 (got {dtype} for a table of {kind})")
-    if wanted and torch.is_grad_enabled():
+    # (inside a level of forward-mode differentiation an input may carry a tangent: torch refuses those, which the function has no rule for)
+    if wanted and torch.is_grad_enabled() or forward_ad._current_level >= 0:
         return _Lookup.apply(table, ids, scale, width, dtype)
     arguments, *keep = _arguments(table, ids, scale, width, dtype)
     return _forward(arguments, ids.shape + shape[1:], dtype, device)
