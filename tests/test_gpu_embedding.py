@@ -491,3 +491,16 @@ def test_forward_mode_tangents_are_refused():
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: embedding.lookup(t, ids, scale), (table,), (table,))
     assert torch.equal(embedding.lookup(table, ids, scale), want)
+
+
+@pytest.mark.parametrize("clipped", [False, True])
+def test_a_step_between_forward_and_backward_is_noticed(clipped):
+    """The scales' gradient reads the table: stepped in between, it is not the table that the result was looked up in."""
+    from vegs_amd import embedding, optim
+    table, ids, scale, g = _inputs(300, 30, 45, "holes", seed=11)
+    t, s = torch.nn.Parameter(table), scale.requires_grad_(True)
+    t.grad = torch.ones_like(t)
+    y = embedding.lookup(t, ids, s)
+    optim.step_many([optim.Adam([t], lr=0.1)], max_grad_norm=1.0 if clipped else None)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [s], g)

@@ -490,3 +490,55 @@ def test_gradients_that_share_a_part_of_their_memory_are_refused(error_if_nonfin
     assert torch.equal(b, before)
     want = _norm64([before[:6000], before[5999:]])
     assert abs(optim.grad_norm([_param(b[:6000]), _param(b[5999:])]).item() - want) <= 2.0 ** -24 * 1.01 * want
+
+
+def test_what_the_kernels_write_has_a_new_version():
+    """As after torch's own clipping and Adam: a graph that needs the old values raises."""
+    from vegs_amd import optim
+    g, = _make([(40, 3)], seed=1)
+    for grad in (g, _make([(40, 6)], seed=1)[0][:, ::2]):
+        p = torch.empty((40, 3), device=DEV)
+        p.grad = grad
+        w = torch.ones((40, 3), device=DEV, requires_grad=True)
+        y = (p.grad * w).sum()                        # its backward reads p.grad
+        optim.grad_norm(p)
+        assert torch.autograd.grad(y, [w], retain_graph=True)[0].equal(p.grad)
+        optim.clip_grad_norm_(p, 0.5)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, [w])
+    opt = optim.Adam([{"params": [torch.nn.Parameter(torch.ones(s, device=DEV))], "name": n}
+                      for n, s in (("a", (50, 1, 3)), ("b", (50, 15, 3)), ("c", (50, 3)))], lr=1e-2)
+    a, b, c = _params([opt])
+
+    def raises(p, step):
+        before = p.detach().clone()
+        y = (p * p).sum()
+        step()
+        assert not torch.equal(p, before)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+    for kw in ({}, {"max_grad_norm": 1.0}):
+        c.grad = torch.ones_like(c)
+        raises(c, lambda: optim.step_many([opt], **kw))
+        raises(c, opt.step)
+        c.grad = None
+        means, factors = torch.zeros(50, 3, device=DEV), torch.ones(1, 50, 3, device=DEV)
+        campos = torch.ones(1, 3, device=DEV)
+        for p in (a, b):
+            raises(p, lambda: optim.adam_step_sh_factored(opt, a, b, means, campos, factors, 3, **kw))
+            versions = [opt.state[p][k]._version for k in ("exp_avg", "exp_avg_sq")]
+            optim.adam_step_sh_factored(opt, a, b, means, campos, factors, 3, **kw)
+            assert all(opt.state[p][k]._version > v for k, v in zip(("exp_avg", "exp_avg_sq"), versions))
+
+
+def test_gradients_and_parameters_of_inference_mode():
+    """They have no version to raise.  (The factor is not a half: 0.5 norm / (norm + 1e-6), 6.5e-8 less of it.)"""
+    from vegs_amd import optim
+    with torch.inference_mode():
+        p = torch.ones(30, device=DEV)
+        p.grad = torch.full((30,), 2.0, device=DEV)
+        plain = _param(torch.full((30,), 2.0, device=DEV))
+        optim.clip_grad_norm_([p, plain], 0.5 * math.sqrt(240.0))
+    before = torch.full((30,), 2.0, device=DEV)
+    _check_clipped([before, before], [p.grad, plain.grad], math.sqrt(240.0), 0.5 * math.sqrt(240.0))

@@ -87,6 +87,15 @@ def _advance(step):
 _ADAM = struct.Struct("4Qqdqd")           # VrAdamTensor
 
 
+def _written(tensors):
+    """Raises the version of tensors that a kernel writes through their addresses, as torch's in-place operations do: a graph
+    that still needs the old values raises in its backward instead of computing on with the new ones."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:                              # (inference tensors have none)
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _grads_of(parameters):
     """The gradients of `parameters` -- a tensor, an optimizer, or an iterable of either -- each one once."""
     if isinstance(parameters, (torch.Tensor, torch.optim.Optimizer)):
@@ -215,6 +224,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             copies.append((g, grads[i]))
     table, device = _grad_table(grads)
     lib = _capi.load()
+    _written(grads)
     with _capi.on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
         scratch = _scratch(lib, len(grads), 0, device)
@@ -269,7 +279,7 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
         for device in devices if grad_norm is not None else ():
             _check_norm(grad_norm, device)
         norm = grad_norm if grad_norm is not None else _norm_of(_once([g for _, entries in batch for _, g, _, _ in entries]), 2)
-    by_cfg, keep = {}, []
+    by_cfg, keep, written = {}, [], []
     for opt, entries in batch:
         for p, g, group, st in entries:
             if st is None:
@@ -282,9 +292,12 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
                 g = g.contiguous()
                 keep.append(g)
             b1, b2 = group["betas"]
+            m, v = st["exp_avg"], st["exp_avg_sq"]
+            written += (p, m, v)
             by_cfg.setdefault((p.device, float(b1), float(b2)), []).append(
-                _ADAM.pack(p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), p.numel(),
+                _ADAM.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
                            float(group["lr"]), _advance(st["step"]), float(group["eps"])))
+    _written(written)
     for (device, b1, b2), items in by_cfg.items():
         with _capi.on(device):
             if norm is None:
@@ -540,7 +553,7 @@ def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, fact
         max_grad_norm = _check_max_norm(max_grad_norm)
     P, n, means3D, campos, factors, fstride = _check_factor_inputs(means3D, campos, factors)
     M = features_dc.shape[1] + (features_rest.shape[1] if features_rest is not None else 0)
-    items, states, betas, eps = [], [], None, None
+    items, states, written, betas, eps = [], [], [], None, None
     for p in (features_dc, features_rest):
         if p is None:
             items.append(None)
@@ -555,6 +568,7 @@ def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, fact
         items.append(_capi.VrShAdamTensor(p.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
                                           float(group["lr"]), int(st["step"].item()) + 1))
         states.append(st)
+        written += (p, st["exp_avg"], st["exp_avg_sq"])
     K = (int(sh_degree) + 1) ** 2
     if not 0 <= int(sh_degree) <= 3 or M < K:
         raise ValueError(f"sh_degree {sh_degree} needs {K} coefficients, the parameters hold {M}")
@@ -566,6 +580,7 @@ def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, fact
         norm = grad_norm if grad_norm is not None else _norm_of((), 2, [(means3D, campos, factors, sh_degree, scale)])
     args = (_capi.ptr(means3D), P, _capi.ptr(campos), _capi.ptr(factors), n, fstride, int(sh_degree), int(M), float(scale),
             C.byref(items[0]), C.byref(items[1]) if items[1] is not None else None, betas[0], betas[1], eps)
+    _written(written)
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev).cuda_stream
         if norm is None:
