@@ -131,3 +131,11 @@ def test_c_entries_refuse_to_scale_shared_memory():
         t, n = table(*entries)
         for rc in (lib.vr_clip_grads(t, n, some, 1.0, None), lib.vr_clip_grad_norm(t, n, 2, 1.0, some, some, None)):
             assert rc == -1 and b"share memory" in lib.vr_last_error()
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("bound", [-1.0, math.nan])
+def test_the_trainer_refuses_a_bad_bound_before_anything_else(bound, fused):
+    from vegs_amd import iteration
+    with pytest.raises(ValueError, match="max_norm"):
+        iteration.Trainer(None, torch.device("cpu"), fused=fused, max_grad_norm=bound)

@@ -220,15 +220,16 @@ class Trainer:
         thousand rows are rebuilt densely (optim.sh_grad_from_factors on their world-space means).
         optimise_boxes: the instances are InstanceModels with their own optimizers and BoxModels with learnable pose
         corrections, all stepped every iteration (train.py:254-275); False keeps them as plain leaf tensors (gradients only).
-        max_grad_norm: clip what every optimizer steps with to this global norm (static model, instance models, pose
-        corrections together; after the exchange, so every rank clips by the same factor).  The fused variant applies the
+        max_grad_norm: clip the loss' gradients, what every optimizer steps with, to this global norm (static model, instance
+        models, pose corrections together; after the exchange, so every rank clips by the same factor).  The poses' second step of
+        the iteration, on their regulariser alone (train.py:274), is neither in the norm nor clipped.  The fused variant applies the
         factor inside the Adam launches -- a factored SH gradient enters the norm from its factors --, the op-by-op one calls
         torch.nn.utils.clip_grad_norm_.  The norm of the last iteration: self.last["grad_norm"].
         world / rank / group: the view-sharded job; exchange: "factored" (default: forces factored_sh), "dense", or
         "direct" (vegs_amd.xgmi: hand-written peer-to-peer exchange)."""
         from . import optim
         self.device, self.fused = device, fused
-        self.max_grad_norm = max_grad_norm
+        self.max_grad_norm = None if max_grad_norm is None else optim._check_max_norm(max_grad_norm)
         self.world, self.rank, self.group, self.exchange = int(world), int(rank), group, exchange
         if exchange not in ("factored", "dense", "direct"):
             raise ValueError(f"exchange must be 'factored', 'dense' or 'direct' (got {exchange!r})")
