@@ -504,3 +504,18 @@ def test_a_step_between_forward_and_backward_is_noticed(clipped):
     optim.step_many([optim.Adam([t], lr=0.1)], max_grad_norm=1.0 if clipped else None)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y, [s], g)
+
+
+@pytest.mark.parametrize("value", [1.9876709, 1.02771, 0.1, 1.0])
+def test_equal_entries_of_one_row_add_up(value):
+    """2^21 entries of one row, equal values, whose roundings do not cancel.  At this width a chunk has 64 entries (64 additions), 16
+    groups join 2048 pieces each, 128 in a row and then 16 such sums, and are added pairwise: 64 + 128 + 16 + 4, and one for the product."""
+    from vegs_amd import embedding
+    n, width = 1 << 21, 130
+    table = torch.zeros((3, width), device=DEV, requires_grad=True)
+    g = torch.full((n, width), value, device=DEV)
+    out = embedding.lookup(table, torch.ones(n, dtype=torch.int32, device=DEV))
+    d, = torch.autograd.grad(out, [table], g)
+    want = n * float(torch.tensor(value, dtype=F32))
+    assert (d[0] == 0).all() and (d[2] == 0).all()
+    assert ((d[1].double() - want).abs() <= (64 + 128 + 16 + 4 + 1) * u * want).all()

@@ -577,8 +577,10 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 
 // Rows that cross borders of chunks: tail[c] + head[c + 1] + ... + head[end].  A workgroup looks at up to JOIN_CHUNKS chunks; short
 // rows are one group's each, rows of more than JOIN_LONG pieces the whole workgroup's: group k adds the pieces k, k + groups, ... and
-// the groups' sums are added pairwise.
-constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 16, JOIN_AHEAD = 8;
+// the groups' sums are added pairwise.  A group adds at most JOIN_RUN pieces in a row, then at most JOIN_RUN such sums, then those: with
+// the 64 entries of a chunk and the 10 steps between 1024 groups at most 394 additions lie between an entry and the result, for the
+// 2^20 pieces a group that 2^30 entries of one row make as well.  (One running sum: 511 u off after 2^21 equal entries, 35 u like this.)
+constexpr int JOIN_THREADS = 1024, JOIN_CHUNKS = 64, JOIN_LONG = 16, JOIN_AHEAD = 8, JOIN_RUN = 128;
 
 // The sums of a workgroup's groups, pairwise: group 0's lanes hold the result.  part: V floats for every thread, free before.
 template <int V>
@@ -600,11 +602,17 @@ __device__ __forceinline__ void add_groups(float (&acc)[V], float* part, int g_s
     }
 }
 
-// acc += the pieces p, p + step, ... up to `end` of the row whose tail is piece c, JOIN_AHEAD of them in flight
-template <int V>
+// acc += the pieces p, p + step, ... up to `end` of the row whose tail is piece c, JOIN_AHEAD of them in flight.  RUNS: any number of
+// them, in runs of JOIN_RUN.
+template <int V, bool RUNS>
 __device__ __forceinline__ void join_pieces(float (&acc)[V], const float* __restrict__ slots, long width, long c, long p, long end,
                                             long step)
 {
+    float runs[V], sums[V];
+    int in_run = JOIN_RUN / JOIN_AHEAD, in_runs = JOIN_RUN;
+#pragma unroll
+    for (int v = 0; v < V; ++v) runs[v] = sums[v] = 0.0f;
+#pragma unroll 1
     for (; p <= end; p += JOIN_AHEAD * step) {
         Pack<float, V> h[JOIN_AHEAD];
 #pragma unroll
@@ -617,11 +625,26 @@ __device__ __forceinline__ void join_pieces(float (&acc)[V], const float* __rest
             if (p + x * step <= end)
 #pragma unroll
                 for (int v = 0; v < V; ++v) acc[v] += h[x].v[v];
+        if (RUNS && --in_run == 0) {
+            in_run = JOIN_RUN / JOIN_AHEAD;
+#pragma unroll
+            for (int v = 0; v < V; ++v) { runs[v] += acc[v]; acc[v] = 0.0f; }
+            if (--in_runs == 0) {
+                in_runs = JOIN_RUN;
+#pragma unroll
+                for (int v = 0; v < V; ++v) { sums[v] += runs[v]; runs[v] = 0.0f; }
+            }
+        }
+    }
+    if (RUNS) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = sums[v] + (runs[v] + acc[v]);
     }
 }
 
+// (V == 4: registers for two workgroups on a CU, which the compiler does not keep to by itself)
 template <typename TT, int V>
-__global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumArgs q, long chunks, int each)
+__global__ void __launch_bounds__(JOIN_THREADS, V == 4 ? 8 : 4) k_lookup_join(LookupArgs a, SumArgs q, long chunks, int each)
 {
     __shared__ long from[JOIN_CHUNKS], upto[JOIN_CHUNKS];
     __shared__ uint32_t row[JOIN_CHUNKS];
@@ -690,7 +713,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        join_pieces<V>(acc, slots, a.width, c, c, end, 1);
+        join_pieces<V, false>(acc, slots, a.width, c, c, end, 1);
         store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
     }
     for (int o = 0; o < count; ++o) {
@@ -699,7 +722,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_lookup_join(LookupArgs a, SumA
         float acc[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-        join_pieces<V>(acc, slots, a.width, c, c + group, end, groups);
+        join_pieces<V, true>(acc, slots, a.width, c, c + group, end, groups);
         __syncthreads();
         add_groups<V>(acc, part, q.g_shift);
         if (group == 0 && live) store_row<TT, V>(d_table + (long)row[o] * a.width, acc);
@@ -862,10 +885,10 @@ static Tiling tiling(int64_t n, int64_t width, int v_full)
     while (t.g_shift < 6 && (1 << t.g_shift) < lanes) ++t.g_shift;
     t.tiles = (int)((lanes + 63) / 64);
     // long chunks make few slots; shorter ones while there are fewer than four waves for each of the 1024 SIMDs (16384 entries of 1024
-    // 16-bit values: 13 us with four, 19 with one) -- but no more than 128 for each group of a join, which is what a row that all
-    // entries hit takes there one after the other
+    // 16-bit values: 13 us with four, 19 with one) -- but not so short that a row that all entries hit has more than JOIN_RUN pieces
+    // for each group of a join, which takes them one after the other (at 64 entries, of more than 8192 a group, it has)
     t.chunk = 64;
-    const int64_t most = 128 * (JOIN_THREADS >> t.g_shift);
+    const int64_t most = JOIN_RUN * (JOIN_THREADS >> t.g_shift);
     while (t.chunk > UNROLL && ((n << t.g_shift) / 64 / t.chunk) * t.tiles < 4096 && 2 * n <= most * t.chunk) t.chunk >>= 1;
     t.chunks = (long)((n + t.chunk - 1) / t.chunk);
     return t;
