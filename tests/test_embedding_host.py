@@ -101,3 +101,19 @@ def test_gradients_of_no_entries_do_not_end_the_process():
                        env=dict(os.environ, HIP_VISIBLE_DEVICES="-1", ROCR_VISIBLE_DEVICES="-1"))
     assert r.returncode == 0, (r.returncode, r.stdout[-500:], r.stderr[-2000:])
     assert [line.split()[2] for line in r.stdout.split("\n") if line] == ["0"] * 6       # the scales' gradient of no entries: nothing to do
+
+
+def test_the_widest_row():
+    """2^22 values; with strides that would take more, so that it is the width that is refused."""
+    lib = _capi.load()
+    some, most = 1 << 20, 1 << 22
+    for width, ok in ((most, True), (most + 1, False)):
+        assert (lib.vr_lookup_scratch_bytes(5000, 7, width) > 0) == ok
+        wide = _lookup(width=width, table_stride=width + 1, n=0, ids=None)
+        assert lib.vr_lookup_forward(C.byref(wide), None, None) == (0 if ok else -1)
+        assert lib.vr_lookup_backward(C.byref(wide), None, width + 1, None, some, None, 0, None) == (0 if ok else -1)
+        assert ok or b"width" in lib.vr_last_error()
+        wide = _lookup(width=width, table_stride=width + 1)
+        if not ok:
+            assert lib.vr_lookup_forward(C.byref(wide), some, None) == -1
+            assert lib.vr_lookup_backward(C.byref(wide), some, width + 1, some, None, some, 1 << 40, None) == -1

@@ -257,7 +257,7 @@ static int check_grads(const VrGradTensor* t, int32_t count)
     for (int i = 0; i < count; ++i) {
         if (t[i].dtype < VR_F32 || t[i].dtype > VR_F16) { set_error("grad norm: tensor %d has an unknown type", i); return VR_ERR_INVALID_ARGUMENT; }
         const uintptr_t element = t[i].dtype == VR_F32 ? 4 : 2;
-        // (one tensor's units are counted in 31 bits: 2^31 x 16 KB)
+        // (one tensor's units are counted in 31 bits: 2^40 values are 2^29 of them)
         if (t[i].n < 0 || (t[i].n > 0 && (!t[i].data || ((uintptr_t)t[i].data & (element - 1)))) || t[i].n > (1ll << 40))
             { set_error("grad norm: tensor %d with NULL or misaligned data or a bad size", i); return VR_ERR_INVALID_ARGUMENT; }
     }
@@ -371,7 +371,7 @@ static int clip_grads(const VrGradTensor* tensors, int32_t count, const float* n
 
 using namespace vr;
 
-// (a launch takes fewer than GN_MAX_T tensors only when its units run out, at 16 TB of gradients)
+// (a launch takes fewer than GN_MAX_T tensors only when its units run out, at 8 TB of gradients)
 extern "C" int64_t vr_grad_norm_scratch_bytes(int32_t count, int32_t n_factors)
 {
     const int64_t launches = (count > 0 ? (count + GN_MAX_T - 1) / GN_MAX_T : 0) + (n_factors > 0 ? n_factors : 0);
