@@ -7,9 +7,10 @@ root=$(git rev-parse --show-toplevel)
 tmp=$(mktemp -d)
 git -C $root archive $commit vegs_amd/csrc include | tar x -C $tmp
 mkdir -p $tmp/obj
+flags=$(cd $root && python -c "from vegs_amd.build import FLAGS; print(*FLAGS)")          # (the shipped library's, so that sources are compared)
 for f in $tmp/vegs_amd/csrc/*.hip; do
   b=$(basename $f .hip)
-  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -munsafe-fp-atomics -fPIC -fno-fast-math -Wno-unused-function -w -c $f -o $tmp/obj/$b.o &
+  /opt/rocm/bin/hipcc $flags -w -c $f -o $tmp/obj/$b.o &
 done
 wait
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 $tmp/obj/*.o -o $root/vegs_amd/_lib/libvegsrast_$name.so

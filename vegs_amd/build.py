@@ -8,6 +8,7 @@ hipcc cross-compiles without a GPU.  Flags that are part of the numerics contrac
                          headline scene: 2.2 % longer).  hipcc's host pass does not know the feature and says so: harmless
 Run:  python -m vegs_amd.build [--force]
 """
+import contextlib
 import os
 import subprocess
 import sys
@@ -61,8 +62,18 @@ def build_variant(name, force=False, verbose=False):
         OBJ_DIR, LIB = keep
 
 
+def _flags_changed():
+    """Whether the objects in OBJ_DIR were compiled with other flags than FLAGS, or with unknown ones."""
+    try:
+        with open(os.path.join(OBJ_DIR, "flags")) as f:
+            return f.read() != " ".join(FLAGS)
+    except OSError:
+        return True
+
+
 def build(force=False, verbose=False, harness=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
+    force = force or _flags_changed()
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
     jobs = []
     for src in SOURCES:
@@ -80,10 +91,16 @@ def build(force=False, verbose=False, harness=True):
         return r.stderr
 
     if jobs:
+        if force:                                        # (known again once every object is new)
+            with contextlib.suppress(FileNotFoundError):
+                os.remove(os.path.join(OBJ_DIR, "flags"))
         with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
             for warn in ex.map(run, jobs):
+                warn = "\n".join(line for line in warn.splitlines() if "'-packed-fp32-ops' is not a recognized feature" not in line)
                 if verbose and warn.strip():
                     print(warn)
+        with open(os.path.join(OBJ_DIR, "flags"), "w") as f:
+            f.write(" ".join(FLAGS))
     objs = [os.path.join(OBJ_DIR, s.replace(".hip", ".o")) for s in SOURCES]
     if force or jobs or _newer(LIB, objs):
         run([_hipcc(), "-shared", "-fPIC", "--offload-arch=gfx950", *objs, "-o", LIB])
