@@ -117,3 +117,11 @@ def test_the_widest_row():
         if not ok:
             assert lib.vr_lookup_forward(C.byref(wide), some, None) == -1
             assert lib.vr_lookup_backward(C.byref(wide), some, width + 1, some, None, some, 1 << 40, None) == -1
+
+
+def test_few_entries_take_no_scratch():
+    """The count up to which the caller does not ask."""
+    lib = _capi.load()
+    for rows, width in ((1, 1), (7, 3), (1 << 20, 4096), (5, 1 << 22)):
+        assert lib.vr_lookup_scratch_bytes(embedding._ALONE, rows, width) == 0
+        assert lib.vr_lookup_scratch_bytes(embedding._ALONE + 1, rows, width) > 0

@@ -519,3 +519,20 @@ def test_equal_entries_of_one_row_add_up(value):
     want = n * float(torch.tensor(value, dtype=F32))
     assert (d[0] == 0).all() and (d[2] == 0).all()
     assert ((d[1].double() - want).abs() <= (64 + 128 + 16 + 4 + 1) * u * want).all()
+
+
+@pytest.mark.parametrize("n", [100, 5000])
+def test_saved_tensors_in_another_order_of_strides(n):
+    """A hook may give back the values laid out otherwise: the gradients are laid out as their inputs' shapes say."""
+    from vegs_amd import embedding
+    table, ids, scale, g = _inputs(n, 40, 12, "holes", whole=True)
+    ids, scale, g = ids.reshape(n // 4, 4), scale.reshape(n // 4, 4), g.reshape(n // 4, 4, 12)
+    want = _run(table, ids, scale, g)
+    turned = lambda x: x.t().contiguous().t()
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: turned(x) if x.dim() == 2 else x):
+        got = _run(table, ids, scale, g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # only the table's: the type of the result is not the table's
+    t = table.bfloat16().requires_grad_(True)
+    d, = torch.autograd.grad(embedding.lookup(t, ids, scale, dtype=F32), [t], g)
+    assert d.dtype == BF16 and d.is_contiguous() and torch.equal(d, want[1].bfloat16())

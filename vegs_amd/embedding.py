@@ -9,7 +9,6 @@ pose corrections by frame.  The table's gradient is dense, in the table's type: 
 vegs_amd.optim.Adam, counted by grad_norm and exchanged by vegs_amd.dist like any other parameter.  GPU tensors only; there
 is no CPU path.
 """
-import math
 import struct
 
 import torch
@@ -36,6 +35,7 @@ def _row_layout(t, lead, width):
 
 
 _LOOKUP = struct.Struct("3Q4q3if")           # VrLookup
+_ALONE = 1024                                # up to so many entries vr_lookup_scratch_bytes is 0
 
 
 def _arguments(table, ids, scale, width, dtype):
@@ -53,52 +53,58 @@ def _arguments(table, ids, scale, width, dtype):
                         kinds[dtype], ids.dtype == torch.int64, scale), table, ids, rows
 
 
-def _forward(arguments, shape, dtype, device):
-    index = device.index
-    if torch.cuda.current_device() != index:
+# (What allocates and where follows the host's time, which is what a call of few ids takes: new_empty and empty_like are half of
+# torch.empty with its keywords, and torch._C._cuda_getDevice a third of torch.cuda.current_device.)
+def _forward(arguments, shape, dtype, table):
+    index = table.get_device()
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
-            return _forward(arguments, shape, dtype, device)
-    out = torch.empty(shape, dtype=dtype, device=device)
+            return _forward(arguments, shape, dtype, table)
+    out = table.new_empty(shape) if dtype is table.dtype else table.new_empty(shape, dtype=dtype)
     if out.numel():
-        rc = (_capi._lib or _capi.load()).vr_lookup_forward(arguments, out.data_ptr(), _capi.stream_of(device))
+        rc = (_capi._lib or _capi.load()).vr_lookup_forward(arguments, out.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
         if rc:
             _capi.check(rc)
     return out
 
 
 def _backward(ctx, g):
-    device, index = g.device, g.get_device()
-    if torch.cuda.current_device() != index:
+    index = g.get_device()
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _backward(ctx, g)
     # (hooks on saved tensors -- recomputation, offloading -- give them back at addresses of their own)
     rows, flat, scales = ctx.saved_tensors
     scale, shape, kind, dtype, ids_shape, n, width = ctx.lookup
-    want_table, _, want_scale, _, _ = ctx.needs_input_grad
+    want_table, _, want_scale, _, _, _ = ctx.needs_input_grad
     d_table = d_scale = scratch = None
     nbytes = at_table = at_scale = 0
     lib = _capi._lib or _capi.load()
     if want_table:
-        d_table = torch.empty(shape, dtype=kind, device=device)
+        if rows is not None and rows.is_contiguous():
+            d_table = torch.empty_like(rows)
+        else:
+            d_table = g.new_empty(shape) if kind is dtype else g.new_empty(shape, dtype=kind)
         at_table = d_table.data_ptr()
-        nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width)
+        if n > _ALONE:
+            nbytes = lib.vr_lookup_scratch_bytes(n, shape[0], width)
     if want_scale:
-        d_scale = torch.empty(ids_shape, dtype=torch.float32, device=device)
+        d_scale = scales.new_empty(ids_shape)
         at_scale = d_scale.data_ptr()
     if width == 0 or n == 0:
-        return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None
+        return (d_table.zero_() if want_table else None), None, (d_scale.zero_() if want_scale else None), None, None, None
     stride = width
     if not g.is_contiguous():
         g, stride = _row_layout(g, len(ids_shape), width)
     if nbytes:
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        scratch = g.new_empty(nbytes, dtype=torch.uint8)
     # (the table's values are only read for the gradient of the scales: where that is not wanted, anything of its shape stands for it)
     arguments, *keep = _arguments(d_table if rows is None else rows, flat, scale if scales is None else scales, width, dtype)
     rc = lib.vr_lookup_backward(arguments, g.data_ptr(), stride, at_table, at_scale, scratch.data_ptr() if nbytes else None, nbytes,
-                                _capi.stream_of(device))
+                                torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _capi.check(rc)
-    return d_table, None, d_scale, None, None
+    return d_table, None, d_scale, None, None, None
 
 
 _backward_once = once_differentiable(_backward)
@@ -107,11 +113,11 @@ _backward_once = once_differentiable(_backward)
 class _Lookup(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, table, ids, scale, width, dtype):
+    def forward(ctx, table, ids, scale, width, dtype, shape):
         arguments, rows, flat, scales = _arguments(table, ids, scale, width, dtype)
         ctx.lookup = None if scales is not None else scale, table.shape, table.dtype, dtype, ids.shape, ids.numel(), width
         ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, flat, scales)
-        return _forward(arguments, ids.shape + table.shape[1:], dtype, table.device)
+        return _forward(arguments, shape, dtype, table)
 
     @staticmethod
     def backward(ctx, g):
@@ -136,7 +142,8 @@ def lookup(table, ids, scale=None, dtype=None):
         raise ValueError(f"table must be a dense float32, bfloat16 or float16 tensor [K, ...] (got {kind} {tuple(shape)})")
     if not isinstance(ids, torch.Tensor) or ids.device != device or ids.dtype not in _ID_TYPES:
         raise ValueError(f"ids must be an int32 or int64 tensor on {device}")
-    width = math.prod(shape[1:])
+    row = shape[1:]
+    width = row.numel()
     if ids.numel() >= 1 << 30 or shape[0] >= (1 << 31) - 1 or width > 1 << 22:
         raise ValueError("at most 2^30 - 1 ids, 2^31 - 2 rows and 2^22 values in a row")
     wanted = table.requires_grad
@@ -155,6 +162,6 @@ def lookup(table, ids, scale=None, dtype=None):
         raise ValueError(f"the result has the table's type or float32 (got {dtype} for a table of {kind})")
     # (inside a level of forward-mode differentiation an input may carry a tangent: torch refuses those, which the function has no rule for)
     if wanted and torch.is_grad_enabled() or forward_ad._current_level >= 0:
-        return _Lookup.apply(table, ids, scale, width, dtype)
+        return _Lookup.apply(table, ids, scale, width, dtype, ids.shape + row)
     arguments, *keep = _arguments(table, ids, scale, width, dtype)
-    return _forward(arguments, ids.shape + shape[1:], dtype, device)
+    return _forward(arguments, ids.shape + row, dtype, table)
