@@ -327,7 +327,7 @@ _HERE_ALREADY = contextlib.nullcontext()
 
 def on(device):
     """torch.cuda.device(device), which is a context of its own only where another device is current."""
-    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE_ALREADY if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def stream_of(device):

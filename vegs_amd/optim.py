@@ -106,19 +106,20 @@ def _grads_of(parameters):
             grads.append(p.grad)
         else:
             grads += [q.grad for group in p.param_groups for q in group["params"]]
-    return _once([g for g in grads if g is not None])
+    return _once(g for g in grads if g is not None)
 
 
 def _once(grads):
-    """Gradients that are the same elements of the same memory, once: the order of the dimensions tells two that fill their memory
-    not apart, but their strides tell two others that begin at one address."""
-    seen = {}
+    """{(address, elements, type): gradient} of gradients that fill their memory, with shape and strides behind these where one does
+    not: each one once.  (The order of the dimensions does not tell two that fill the same memory apart, but the strides tell two
+    others that begin at one address.)"""
+    kinds, seen = _capi.VR_DTYPES, {}
     for g in grads:
         if g.layout is not torch.strided:
             raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.layout})")
-        at, n = g.data_ptr(), g.numel()
-        seen[(at, n, g.dtype) if _dense(g) else (at, n, g.dtype, g.shape, g.stride())] = g
-    return list(seen.values())
+        kind = kinds.get(g.dtype, g.dtype)               # (other types are refused by _grad_table)
+        seen[(g.data_ptr(), g.numel(), kind) if _dense(g) else (g.data_ptr(), g.numel(), kind, g.shape, g.stride())] = g
+    return seen
 
 
 def _dense(t):
@@ -134,18 +135,22 @@ def _dense(t):
     return True
 
 
-def _grad_table(grads):
-    """(flat VrGradTensor words, device) of gradients that fill their memory, checked."""
-    device, kinds = grads[0].device, _capi.VR_DTYPES
-    if not grads[0].is_cuda or len({g.get_device() for g in grads}) != 1:
+def _grad_table(seen):
+    """(flat VrGradTensor words, device, [(gradient, copy of it)]) of what _once returns, checked: gradients that do not fill their
+    memory are copied."""
+    device = next(iter(seen.values())).device
+    if device.type != "cuda" or len({g.get_device() for g in seen.values()}) != 1:
         raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
-    flat = []
-    for g in grads:
-        kind = kinds.get(g.dtype)
-        if kind is None:
-            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.dtype})")
-        flat += (g.data_ptr(), g.numel(), kind)
-    return struct.pack("%dq" % len(flat), *flat), device
+    flat, copies = [], []
+    for key, g in seen.items():
+        if isinstance(key[2], torch.dtype):
+            raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {key[2]})")
+        if len(key) > 3:
+            copy = g.contiguous()
+            copies.append((g, copy))
+            key = (copy.data_ptr(), key[1], key[2])
+        flat += key
+    return struct.pack("%dq" % len(flat), *flat), device, copies
 
 
 def _norm_kind(norm_type):
@@ -181,23 +186,24 @@ def grad_norm(parameters, norm_type=2.0, sh_factors=()):
     return _norm_of(_grads_of(parameters), kind, sh_factors)
 
 
-def _norm_of(grads, kind, sh_factors=()):
-    keep, items = [g if _dense(g) else g.contiguous() for g in grads], []
+def _norm_of(seen, kind, sh_factors=()):
+    items = []
+    table, device, copies = _grad_table(seen) if seen else (None, None, None)
     for means3D, campos, factors, sh_degree, scale in sh_factors:
         P, n, means3D, campos, factors, fstride = _check_factor_inputs(means3D, campos, factors)
-        if keep and means3D.device != keep[0].device or items and means3D.device != items[0][1].device:
+        device = device or means3D.device
+        if means3D.device != device:
             raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
         keep_f = (means3D, campos, factors)
         items.append((_capi.VrShGradFactors(_capi.ptr(means3D), _capi.ptr(campos), _capi.ptr(factors), fstride, P, n,
-                                            int(sh_degree), float(scale)), means3D, keep_f))
-    if not keep and not items:
+                                            int(sh_degree), float(scale)), keep_f))
+    if not seen and not items:
         return torch.tensor(0.0)
-    table, device = _grad_table(keep) if keep else (None, items[0][1].device)
     lib = _capi.load()
     with _capi.on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
-        scratch = _scratch(lib, len(keep), len(items), device)
-        _capi.check(lib.vr_grad_norm(table, len(keep), (_capi.VrShGradFactors * len(items))(*[i[0] for i in items]) if items else None,
+        scratch = _scratch(lib, len(seen), len(items), device)
+        _capi.check(lib.vr_grad_norm(table, len(seen), (_capi.VrShGradFactors * len(items))(*[i[0] for i in items]) if items else None,
                                      len(items), kind, norm.data_ptr(), scratch.data_ptr(), _capi.stream_of(device)))
     return norm
 
@@ -215,16 +221,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     grads = _grads_of(parameters)
     if not grads:
         return torch.tensor(0.0)
-    copies = []
-    for i, g in enumerate(grads):
-        if not _dense(g):
-            if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-                raise ValueError("an expanded gradient (one value in memory for several elements) cannot be clipped in place")
-            grads[i] = g.contiguous()
-            copies.append((g, grads[i]))
-    table, device = _grad_table(grads)
+    table, device, copies = _grad_table(grads)
+    for g, _ in copies:
+        if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+            raise ValueError("an expanded gradient (one value in memory for several elements) cannot be clipped in place")
     lib = _capi.load()
-    _written(grads)
     with _capi.on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
         scratch = _scratch(lib, len(grads), 0, device)
@@ -234,8 +235,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             if not math.isfinite(norm.item()):
                 raise RuntimeError(f"the total norm of order {float(norm_type)} of the gradients is not finite, so they cannot be "
                                    "clipped; error_if_nonfinite=False scales them all the same")
+            _written(list(grads.values()))
             rc = lib.vr_clip_grads(table, len(grads), norm.data_ptr(), max_norm, stream)
         else:
+            _written(list(grads.values()))
             rc = lib.vr_clip_grad_norm(table, len(grads), kind, max_norm, norm.data_ptr(), scratch.data_ptr(), stream)
     if rc == _capi.INVALID_ARGUMENT:                  # (what is left for the library to refuse: shared memory)
         raise ValueError(lib.vr_last_error().decode())
@@ -278,7 +281,7 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
             raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
         for device in devices if grad_norm is not None else ():
             _check_norm(grad_norm, device)
-        norm = grad_norm if grad_norm is not None else _norm_of(_once([g for _, entries in batch for _, g, _, _ in entries]), 2)
+        norm = grad_norm if grad_norm is not None else _norm_of(_once(g for _, entries in batch for _, g, _, _ in entries), 2)
     by_cfg, keep, written = {}, [], []
     for opt, entries in batch:
         for p, g, group, st in entries:
@@ -577,7 +580,7 @@ def adam_step_sh_factored(opt, features_dc, features_rest, means3D, campos, fact
     if max_grad_norm is not None:
         if grad_norm is not None:
             _check_norm(grad_norm, dev)
-        norm = grad_norm if grad_norm is not None else _norm_of((), 2, [(means3D, campos, factors, sh_degree, scale)])
+        norm = grad_norm if grad_norm is not None else _norm_of({}, 2, [(means3D, campos, factors, sh_degree, scale)])
     args = (_capi.ptr(means3D), P, _capi.ptr(campos), _capi.ptr(factors), n, fstride, int(sh_degree), int(M), float(scale),
             C.byref(items[0]), C.byref(items[1]) if items[1] is not None else None, betas[0], betas[1], eps)
     _written(written)
