@@ -28,14 +28,14 @@ struct LookupArgs {
 template <typename T, int V>
 struct __attribute__((packed)) Pack { T v[V]; };
 
-// 16 bytes at an address of 2 or 4 bytes' alignment, past the caches' normal order of replacement
+// 16 bytes at an address of 2 or 4 bytes' alignment; ONCE: past the caches' normal order of replacement
 typedef uint32_t quad_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t quad_2 __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_once(const T* p)
+template <typename T, int V, bool ONCE>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p)
 {
-    if (sizeof(Pack<T, V>) != 16) return *reinterpret_cast<const Pack<T, V>*>(p);
+    if (!ONCE || sizeof(Pack<T, V>) != 16) return *reinterpret_cast<const Pack<T, V>*>(p);
     using Q = typename std::conditional<sizeof(T) == 4, quad_4, quad_2>::type;
     const Q q = __builtin_nontemporal_load(reinterpret_cast<const Q*>(p));
     Pack<T, V> out;
@@ -446,8 +446,11 @@ __global__ void __launch_bounds__(PASS_THREADS) k_sort_scatter(LookupArgs a, Pas
 // before; tail: of the row that begins here and goes on -- and k_lookup_join adds a row's tail and the heads behind it in order.
 // No atomics, and every order fixed by the sizes and the ids.
 //
-// The gradient rows are gathered: each is one contiguous read of width x 4 bytes, UNROLL of them in flight per lane.
+// The gradient rows are gathered: each is one contiguous read of width x 4 bytes, UNROLL of them in flight per lane.  ONCE: streamed,
+// where the gradient is larger than the 256 MB cache in front of the memory.  (Rows of 45 floats, right after the kernel that wrote them:
+// 54 MB 44 us streamed and 30 as other reads, 108 MB 53 and 33, 180 MB 76 and 66, 360 MB 144 and 149.)
 constexpr int UNROLL = 8;
+constexpr long SUM_ONCE_BYTES = 256l << 20;
 
 struct SumArgs {
     const uint32_t *key, *val;
@@ -461,7 +464,7 @@ struct SumArgs {
     int g_shift;                  // G = 1 << g_shift lanes
 };
 
-template <typename TT, typename TO, int V, bool DSCALE>
+template <typename TT, typename TO, int V, bool DSCALE, bool ONCE>
 __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
 {
     constexpr int U = UNROLL, U_SHIFT = 3;
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(256) k_lookup_sum(LookupArgs a, SumArgs q)
         for (int x = 0; x < U; ++x) {
             const bool there = key[x] < rows;
             s[x] = q.scales ? q.scales[j + x] : there && a.row_scale ? a.row_scale[val[x]] : 1.0f;     // (padded as the keys)
-            g[x] = load_once<TO, V>(grad + (there ? (long)val[x] * q.grad_stride : 0));
+            g[x] = load_pack<TO, V, ONCE>(grad + (there ? (long)val[x] * q.grad_stride : 0));
         }
         float dot[U];
 #pragma unroll
@@ -760,7 +763,7 @@ __device__ __forceinline__ void add_entries(const LookupArgs& a, const SumArgs& 
         for (int x = 0; x < UNROLL; ++x) {
             const long i = val[j + x < end ? j + x : j];
             s[x] = a.row_scale ? a.row_scale[i] : 1.0f;
-            g[x] = load_once<TO, V>(grad + i * q.grad_stride);
+            g[x] = load_pack<TO, V, false>(grad + i * q.grad_stride);
         }
 #pragma unroll
         for (int x = 0; x < UNROLL; ++x) {
@@ -954,6 +957,13 @@ struct Forward {
 
 // Everything after the sort.
 struct Backward {
+    template <typename TT, typename TO, int V, bool ONCE>
+    static void sums(const LookupArgs& a, const SumArgs& q, const Tiling& t, bool fused, hipStream_t s)
+    {
+        const dim3 grid((unsigned)(((t.chunks << t.g_shift) + 255) / 256), t.tiles);
+        if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, true, ONCE>), grid, dim3(256), 0, s, a, q);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, false, ONCE>), grid, dim3(256), 0, s, a, q);
+    }
     template <typename TT, typename TO, int V>
     static void launch(const LookupArgs& a, const SumArgs& q, const Tiling& t, hipStream_t s)
     {
@@ -965,10 +975,10 @@ struct Backward {
             if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_small<TT, TO, V, true>), grid, dim3(SORT_THREADS), 0, s, a, q, key_bits(a.rows), rows_each);
             else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_small<TT, TO, V, false>), grid, dim3(SORT_THREADS), 0, s, a, q, key_bits(a.rows), rows_each);
         } else if (q.d_table) {
-            const dim3 grid((unsigned)(((t.chunks << t.g_shift) + 255) / 256), t.tiles);
-            if (fused) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, true>), grid, dim3(256), 0, s, a, q);
-            else hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_sum<TT, TO, V, false>), grid, dim3(256), 0, s, a, q);
-            // (few chunks: fewer a workgroup, so that each of its groups has one row at most)
+            if (V > 1 && a.n * a.width * (long)sizeof(TO) > SUM_ONCE_BYTES) sums<TT, TO, V, V != 1>(a, q, t, fused, s);
+            else sums<TT, TO, V, false>(a, q, t, fused, s);
+            // (few chunks: fewer a workgroup, so that each of its groups has one row at most.  8125 chunks of 45 floats: 5 us with 16, 8
+            // with 64; 31250: 19 and 13)
             const int each = t.chunks > 8192 ? JOIN_CHUNKS : JOIN_CHUNKS / 4;
             if (t.chunks > 1)
                 hipLaunchKernelGGL(HIP_KERNEL_NAME(k_lookup_join<TT, V>), dim3((unsigned)((t.chunks + each - 1) / each), t.tiles),
