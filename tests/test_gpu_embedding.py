@@ -536,3 +536,16 @@ def test_saved_tensors_in_another_order_of_strides(n):
     t = table.bfloat16().requires_grad_(True)
     d, = torch.autograd.grad(embedding.lookup(t, ids, scale, dtype=F32), [t], g)
     assert d.dtype == BF16 and d.is_contiguous() and torch.equal(d, want[1].bfloat16())
+
+
+@pytest.mark.parametrize("wanted", [False, True])
+def test_numbers_as_scales(wanted):
+    """Float32's range and what float32 has beyond numbers; not what it would have to round to infinity."""
+    from vegs_amd import embedding
+    t, ids = torch.ones(5, 3, device=DEV, requires_grad=wanted), torch.tensor([1, -1], device=DEV)
+    for scale in (0.0, -2, True, 2.0 ** -149, torch.finfo(F32).max, -torch.finfo(F32).max, math.inf, -math.inf, math.nan, np.float32(0.25)):
+        out = embedding.lookup(t, ids, scale).detach()
+        assert torch.equal(out[0].nan_to_num(7.0), torch.full((3,), float(scale), device=DEV).nan_to_num(7.0)) and (out[1] == 0).all()
+    for scale in (1e39, -1e39, 3.5e38, "x"):
+        with pytest.raises(ValueError):
+            embedding.lookup(t, ids, scale)

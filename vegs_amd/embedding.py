@@ -9,6 +9,7 @@ pose corrections by frame.  The table's gradient is dense, in the table's type: 
 vegs_amd.optim.Adam, counted by grad_norm and exchanged by vegs_amd.dist like any other parameter.  GPU tensors only; there
 is no CPU path.
 """
+import math
 import struct
 
 import torch
@@ -35,6 +36,7 @@ def _row_layout(t, lead, width):
 
 
 _LOOKUP = struct.Struct("3Q4q3if")           # VrLookup
+_LARGEST = torch.finfo(torch.float32).max
 _ALONE = 1024                                # up to so many entries vr_lookup_scratch_bytes is 0
 
 
@@ -129,8 +131,8 @@ def lookup(table, ids, scale=None, dtype=None):
     """scale * table[ids]: [*ids.shape, *table.shape[1:]], differentiable with respect to `table` and to a `scale` tensor.
 
     table: [K, ...] float32, bfloat16 or float16.  ids: int32 or int64 of any shape; an id outside [0, K) -- -1 by
-    convention -- means "no row": zeros, and no gradient whatever stands in its place.  scale: a number, or a float32
-    tensor shaped like ids.  dtype: of the result, the table's (default) or float32.
+    convention -- means "no row": zeros, and no gradient whatever stands in its place.  scale: a number of float32's range, or a
+    float32 tensor shaped like ids.  dtype: of the result, the table's (default) or float32.
 
     The product is formed in float32 and rounded once.  The table's gradient adds the entries of a row in float32, in an order
     that the sizes and ids fix, and is rounded once to the table's type; it is dense (rows without an entry are zeros) and the same
@@ -156,6 +158,8 @@ def lookup(table, ids, scale=None, dtype=None):
         wanted = wanted or scale.requires_grad
     else:
         scale = float(scale)
+        if abs(scale) > _LARGEST and scale not in (math.inf, -math.inf):
+            raise ValueError(f"a scale must be a float32 number (got {scale})")
     if dtype is None:
         dtype = kind
     elif dtype != kind and dtype != torch.float32:
