@@ -542,3 +542,21 @@ def test_gradients_and_parameters_of_inference_mode():
         optim.clip_grad_norm_([p, plain], 0.5 * math.sqrt(240.0))
     before = torch.full((30,), 2.0, device=DEV)
     _check_clipped([before, before], [p.grad, plain.grad], math.sqrt(240.0), 0.5 * math.sqrt(240.0))
+
+
+@pytest.mark.parametrize("bound", [None, 1.0])
+def test_a_parameter_met_twice_is_not_stepped_at_all(bound):
+    """One launch would read, step and write it from two workgroups."""
+    from vegs_amd import optim
+    p, q = (torch.nn.Parameter(torch.ones(5000, device=DEV)) for _ in range(2))
+    a, b, c = optim.Adam([p], lr=0.1), optim.Adam([q, p], lr=0.1), optim.Adam([q], lr=0.1)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    for opts in ([a, a], [a, b], [c, b, a]):
+        with pytest.raises(ValueError, match="twice"):
+            optim.step_many(opts, max_grad_norm=bound)
+    assert (p == 1).all() and (q == 1).all() and not a.state and not b.state and not c.state
+    optim.step_many([a, c], max_grad_norm=bound)
+    assert (p < 1).all() and (q < 1).all()
+    q.grad = None                                   # without a gradient it is not stepped, and may be in both
+    optim.step_many([b, c], max_grad_norm=bound)
+    assert float(b.state[p]["step"]) == 1

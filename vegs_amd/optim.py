@@ -274,6 +274,8 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
         max_grad_norm = _check_max_norm(max_grad_norm)
     lib = _capi.load()
     batch = [(opt, _entries(opt)) for opt in optimizers]
+    if len({id(p) for _, entries in batch for p, _, _, _ in entries}) != sum(len(entries) for _, entries in batch):
+        raise ValueError("a parameter is in two of the optimizers, or an optimizer twice in the list: one launch steps each parameter once")
     norm = None
     if max_grad_norm is not None:
         devices = {p.device for _, entries in batch for p, _, _, _ in entries}
