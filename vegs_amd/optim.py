@@ -45,8 +45,8 @@ class Adam(torch.optim.Optimizer):
 
 
 def _entries(optimizer):
-    """[(parameter, gradient, group, its state or None)] of one optimizer (vegs_amd.optim.Adam or torch.optim.Adam: same
-    state layout), parameters without a gradient left out -- with everything checked WITHOUT touching the optimizer: step_many
+    """[(parameter, gradient, group, its state or None, optimizer)] of one optimizer (vegs_amd.optim.Adam or torch.optim.Adam:
+    same state layout), parameters without a gradient left out -- with everything checked WITHOUT touching the optimizer: step_many
     goes through every optimizer of its batch before the first step counter moves, so an exception leaves all of them exactly
     as they were (a half-advanced batch would skew the bias correction of a retry and desynchronise the ranks of a
     distributed job)."""
@@ -70,7 +70,7 @@ def _entries(optimizer):
                 if (m is None or v is None or "step" not in st or m.shape != shape or v.shape != shape
                         or not m.is_contiguous() or not v.is_contiguous()):
                     raise ValueError("optimizer state does not match its parameter")
-            out.append((p, g, group, st))
+            out.append((p, g, group, st, optimizer))
     return out
 
 
@@ -117,8 +117,10 @@ def _once(grads):
     for g in grads:
         if g.layout is not torch.strided:
             raise ValueError(f"gradients must be dense float32, bfloat16 or float16 tensors (got {g.layout})")
-        kind = kinds.get(g.dtype, g.dtype)               # (other types are refused by _grad_table)
-        seen[(g.data_ptr(), g.numel(), kind) if _dense(g) else (g.data_ptr(), g.numel(), kind, g.shape, g.stride())] = g
+        key = g.data_ptr(), g.numel(), kinds.get(g.dtype, g.dtype)               # (other types are refused by _grad_table)
+        if not g.is_contiguous() and not _dense(g):
+            key += g.shape, g.stride()
+        seen[key] = g
     return seen
 
 
@@ -169,8 +171,10 @@ def _check_max_norm(max_norm):
     return max_norm
 
 
-def _scratch(lib, count, n_factors, device):
-    return torch.empty(lib.vr_grad_norm_scratch_bytes(count, n_factors) >> 3, dtype=torch.float64, device=device)
+def _norm_and_scratch(lib, count, n_factors, near):
+    """(a 0-dim float32 tensor, the norm's scratch) on the device of `near`, which is current."""
+    return (near.new_empty((), dtype=torch.float32),
+            near.new_empty(lib.vr_grad_norm_scratch_bytes(count, n_factors) >> 3, dtype=torch.float64))
 
 
 def grad_norm(parameters, norm_type=2.0, sh_factors=()):
@@ -201,8 +205,7 @@ def _norm_of(seen, kind, sh_factors=()):
         return torch.tensor(0.0)
     lib = _capi.load()
     with _capi.on(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        scratch = _scratch(lib, len(seen), len(items), device)
+        norm, scratch = _norm_and_scratch(lib, len(seen), len(items), next(iter(seen.values())) if seen else means3D)
         _capi.check(lib.vr_grad_norm(table, len(seen), (_capi.VrShGradFactors * len(items))(*[i[0] for i in items]) if items else None,
                                      len(items), kind, norm.data_ptr(), scratch.data_ptr(), _capi.stream_of(device)))
     return norm
@@ -227,8 +230,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             raise ValueError("an expanded gradient (one value in memory for several elements) cannot be clipped in place")
     lib = _capi.load()
     with _capi.on(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        scratch = _scratch(lib, len(grads), 0, device)
+        norm, scratch = _norm_and_scratch(lib, len(grads), 0, next(iter(grads.values())))
         stream = _capi.stream_of(device)
         if error_if_nonfinite:
             _capi.check(lib.vr_grad_norm(table, len(grads), None, 0, kind, norm.data_ptr(), scratch.data_ptr(), stream))
@@ -273,37 +275,35 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
     else:
         max_grad_norm = _check_max_norm(max_grad_norm)
     lib = _capi.load()
-    batch = [(opt, _entries(opt)) for opt in optimizers]
-    if len({id(p) for _, entries in batch for p, _, _, _ in entries}) != sum(len(entries) for _, entries in batch):
+    batch = [entry for opt in optimizers for entry in _entries(opt)]
+    if len({id(entry[0]) for entry in batch}) != len(batch):
         raise ValueError("a parameter is in two of the optimizers, or an optimizer twice in the list: one launch steps each parameter once")
     norm = None
     if max_grad_norm is not None:
-        devices = {p.device for _, entries in batch for p, _, _, _ in entries}
-        if len(devices) > 1:
-            raise ValueError("gradients to be clipped together must be GPU tensors on one device (there is no CPU path)")
-        for device in devices if grad_norm is not None else ():
-            _check_norm(grad_norm, device)
-        norm = grad_norm if grad_norm is not None else _norm_of(_once(g for _, entries in batch for _, g, _, _ in entries), 2)
+        if grad_norm is not None:
+            for entry in batch:
+                _check_norm(grad_norm, entry[0].device)
+        norm = grad_norm if grad_norm is not None else _norm_of(_once([entry[1] for entry in batch]), 2)
     by_cfg, keep, written = {}, [], []
-    for opt, entries in batch:
-        for p, g, group, st in entries:
-            if st is None:
-                st = opt.state[p]
-                if len(st) == 0:
-                    st["step"] = torch.tensor(0.0, dtype=torch.float32)
-                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            b1, b2 = group["betas"]
-            m, v = st["exp_avg"], st["exp_avg_sq"]
-            written += (p, m, v)
-            by_cfg.setdefault((p.device, float(b1), float(b2)), []).append(
-                _ADAM.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
-                           float(group["lr"]), _advance(st["step"]), float(group["eps"])))
+    for p, g, group, st, opt in batch:
+        if st is None:
+            st = opt.state[p]
+            if len(st) == 0:
+                st["step"] = torch.tensor(0.0, dtype=torch.float32)
+                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        b1, b2 = group["betas"]
+        m, v = st["exp_avg"], st["exp_avg_sq"]
+        written += (p, m, v)
+        by_cfg.setdefault((p.get_device(), float(b1), float(b2)), []).append(
+            _ADAM.pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
+                       float(group["lr"]), _advance(st["step"]), float(group["eps"])))
     _written(written)
-    for (device, b1, b2), items in by_cfg.items():
+    for (index, b1, b2), items in by_cfg.items():
+        device = torch.device("cuda", index)
         with _capi.on(device):
             if norm is None:
                 rc = lib.vr_adam_step(b"".join(items), len(items), b1, b2, -1.0, _capi.stream_of(device))
