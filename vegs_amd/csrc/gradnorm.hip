@@ -3,7 +3,7 @@
 //   norm = sqrt(sum over all tensors of g^2)   or   max |g|;      g *= min(1, max_norm / (norm + 1e-6))
 //
 // Bound by HBM: the norm reads every gradient once, the scaling reads and writes it once more, and only when the factor is not
-// one (118 M fp32 elements: 76 us, 6.2 TB/s, and 152 us, 6.2 TB/s).  The squares are taken and added in fp64: a product of two
+// one (118 M fp32 elements: 76 us, 6.2 TB/s, and 150 us, 6.3 TB/s).  The squares are taken and added in fp64: a product of two
 // fp32 values is exact there and neither overflows nor vanishes, and the vector ALUs do 64-bit multiply-adds an order of
 // magnitude faster than memory delivers operands.  No atomics: every workgroup writes one partial result, and they are added in
 // one fixed order, so that the ranks of a job that hold the same gradients clip by the same bits.
@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(256) k_grad_norm(GradArgs a, double* __restric
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
-// (2 M Gaussians, degree 3: 22 us for one view, 41 for four; the dense gradient would be 384 MB to write and read.)
+// (2 M Gaussians, degree 3: 22 us for one view, 41 for four, where the bytes take 9 and 23 at a copy's rate: one Gaussian's loads in
+// flight a thread, and the 48 squares one after the other; the dense gradient would be 384 MB to write and read.)
 // One Gaussian per thread: its dense SH row is rebuilt in registers, from the same function the optimizer's kernel
 // steps with, and only its squares leave.
 template <bool MAX>

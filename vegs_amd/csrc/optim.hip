@@ -47,8 +47,8 @@ __device__ __forceinline__ void adam_elem(float& p, float g, float& m, float& v,
 
 // CLIP: every gradient is multiplied by clip_factor(*norm, max_norm) where it is loaded -- the clipped gradients of
 // vr_clip_grads without their 12 bytes per element (read, write, read again); a factor of one leaves the step bit for bit.
-// 118 M elements: 512 us (6.45 TB/s), as the step without it; the norm before it another 80.  (Running the blocks from the last to the
-// first, for the 256 MB of gradients that the norm read last and the memory-side cache may hold, changes nothing: 512.)
+// 118 M elements: 531 us (6.2 TB/s; 513 at best), as the step without it; the norm before it another 80.  (Running the blocks from the
+// last to the first, for the 256 MB of gradients that the norm read last and the memory-side cache may hold, changes nothing.)
 template <bool CLIP>
 __global__ void __launch_bounds__(256) k_adam(AdamArgs a)
 {
