@@ -549,3 +549,19 @@ def test_numbers_as_scales(wanted):
     for scale in (1e39, -1e39, 3.5e38, "x"):
         with pytest.raises(ValueError):
             embedding.lookup(t, ids, scale)
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+def test_tangents_that_arrive_in_the_backward_are_refused(by_row):
+    """Forward over reverse: what follows the lookup carries a tangent, and so does the gradient that reaches it."""
+    import torch.autograd.forward_ad as fwd
+    from vegs_amd import embedding
+    table, ids, scale, g = _inputs(50, 9, 5, "holes", scale="row" if by_row else 2.0, seed=2)
+    table.requires_grad_(True)
+    with fwd.dual_level():
+        out = embedding.lookup(table, ids, scale)
+        weighted = (out * fwd.make_dual(g, torch.ones_like(g))).sum()
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(weighted, [table])
+        d, = torch.autograd.grad((embedding.lookup(table, ids, scale) * g).sum(), [table])
+    assert torch.equal(d, torch.autograd.grad((embedding.lookup(table, ids, scale) * g).sum(), [table])[0])

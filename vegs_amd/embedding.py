@@ -75,6 +75,8 @@ def _backward(ctx, g):
     if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _backward(ctx, g)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(g).tangent is not None:
+        raise NotImplementedError("the gradients of lookup have no forward-mode derivative")
     # (hooks on saved tensors -- recomputation, offloading -- give them back at addresses of their own)
     rows, flat, scales = ctx.saved_tensors
     scale, shape, kind, dtype, ids_shape, n, width = ctx.lookup
