@@ -281,8 +281,8 @@ def step_many(optimizers, max_grad_norm=None, grad_norm=None):
     norm = None
     if max_grad_norm is not None:
         if grad_norm is not None:
-            for entry in batch:
-                _check_norm(grad_norm, entry[0].device)
+            for index in {entry[0].get_device() for entry in batch}:
+                _check_norm(grad_norm, torch.device("cuda", index))
         norm = grad_norm if grad_norm is not None else _norm_of(_once([entry[1] for entry in batch]), 2)
     by_cfg, keep, written = {}, [], []
     for p, g, group, st, opt in batch:
